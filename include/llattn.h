@@ -83,6 +83,16 @@ int llattn_qkv_prepare_commit(const float* qkv, const int32_t* pos, const float*
                               const float* inv_freq, void* q, void* k, void* v, int nb, void* cache, const int32_t* pages,
                               int max_blocks, int blk, void* stream);
 
+/* The same two with several position axes, for tokens of images and video (time, height, width): pos is [naxes][T], 1 to
+ * LLATTN_MAX_AXES axes, and frequency i turns by the position on axis axis_of[i] (a HOST array of 32 axes, read during the call). A token
+ * with one position on all axes gets the bits of the one-axis entry points. No counterpart in the reference, whose tokens are text. */
+#define LLATTN_MAX_AXES 4
+int llattn_qk_norm_rope_axes(const float* qkv, const int32_t* pos, int naxes, const uint8_t* axis_of, const float* gq, const float* gk,
+                             float eps, const float* inv_freq, void* q, void* k, void* v, int T, void* stream);
+int llattn_qkv_prepare_commit_axes(const float* qkv, const int32_t* pos, int naxes, const uint8_t* axis_of, const float* gq, const float* gk,
+                                   float eps, const float* inv_freq, void* q, void* k, void* v, int nb, void* cache, const int32_t* pages,
+                                   int max_blocks, int blk, void* stream);
+
 /* ---- consumer of the attention output: the dense projection on the int8 `Act` the attention epilogue writes.
  * Stands in for Engine::gemm<4, 2>(Ly.dense, items_dense, ..., oA.a, ones, HID, HID, nullptr, h, 1, 2)
  * (engine/engine.cu:434 -> moe8::gemm<4, 4, 2, 2>, engine/moe_i8.cu:295-442) for any number of tokens:
@@ -114,6 +124,46 @@ int llattn_dense_status(void* stream, int* code);
 /* The device address of that word on the current device, for a caller that copies it out with its results (a captured
  * graph has no place for llattn_dense_status). */
 int llattn_dense_error_word(int** word);
+
+/* Types of 16- and 32-bit operands where an entry point takes more than one. */
+#define LLATTN_F32 0
+#define LLATTN_F16 1
+#define LLATTN_BF16 2
+
+/* ---- residual addition, norm and int8 activations: what stands in front of a projection.
+ *   v = x + delta (fp32; x <- v),  r = 1 / sqrt(mean(v^2) + eps),  t = v * gain;  for each group of 128 values of a row:
+ *   e = max(max|t| / 127, 1e-30),  q = rint(t / e),  s = e * r,  sum = sum of the codes;  y = t * r, rounded once to 16 bits.
+ * q [T][K], s and sum [T][K/128] are the triple llattn_dense_w4a8 reads (q in fragment order), y [T][K] is fp16 or bf16 (y_type); either may be
+ * NULL, not both. x is fp32, rows ldx values apart; delta (NULL: nothing is added, x is only read) is fp32, fp16 or bf16 (delta_type), rows ldd
+ * values apart. K is a multiple of 128 up to 32,768; ldx and ldd are multiples of 4; x, delta, gain, q and y are 16-byte aligned. No output may
+ * overlap another argument. The codes and sums are the same bits whatever T and the launch. A group that holds an infinity or NaN has codes
+ * 0 and the scale NaN, and NaN anywhere in a row makes all of its scales NaN, so that a projection of it is NaN. A sum of squares beyond fp32
+ * (values around 1e19) gives r = 0. The model's own norm rotates too (engine/ops.cu:116-135); no counterpart of this plain form there. */
+int llattn_add_norm_q8(float* x, int64_t ldx, const void* delta, int delta_type, int64_t ldd, const float* gain, float eps, int8_t* q,
+                       float* s, int32_t* sum, void* y, int y_type, int T, int K, void* stream);
+
+/* ---- low-rank adapters of many requests, beside the projection that they share. No counterpart in the reference.
+ * A pool holds n adapters of one part of a projection's output, the rows [row0, row0 + rows): A [n][rank][K] and B [n][rows][rank], fp16 or bf16
+ * (type); scale [n] fp32 (NULL: 1); ranks [n] (NULL: all of them have `rank`), of which adapter a uses the first ranks[a] rows of A and columns of
+ * B, whatever stands behind them. rank is a multiple of 8 up to 128; rows and row0 are multiples of 4. All four are device memory. */
+typedef struct llattn_adapter_pool {
+    const void* A;
+    const void* B;
+    const float* scale;
+    const int32_t* ranks;
+    int32_t n, rank, rows, row0, type;
+} llattn_adapter_pool;
+#define LLATTN_MAX_ADAPTER_POOLS 4
+
+/* The tokens [seg_first[i], seg_first[i + 1]) belong to segment i, whose adapter is seg_adapter[i] in every pool (both device arrays, nseg + 1
+ * and nseg long, bounds ascending; -1, or an index that the pool does not have: none). For a token n of a segment with adapter a, and every pool:
+ *   Y[n][row0 + i] += scale[a] * sum_j B[a][i][j] * sum_k A[a][j][k] * s[n][k / 128] * q[n][k]
+ * from the activations (q, s) that the projection itself reads, added in fp32; the order of the sums, and so the bits, depends on the sizes only.
+ * Y has ldy values a row (a multiple of 4, at least row0 + rows); tokens outside the segments, and of a segment without an adapter, keep
+ * theirs. `pools` is a host array of 1 to 4 pools of one type whose rows do not overlap (the q, k and v parts of one projection, say), read
+ * during the call; what is on the device may change between replays of a captured call. */
+int llattn_adapters_w4a8(const llattn_adapter_pool* pools, int npools, const int8_t* q, const float* s, float* Y, int64_t ldy, int ntokens,
+                         int K, const int32_t* seg_first, const int32_t* seg_adapter, int nseg, void* stream);
 
 /* ---- the reference operator pair on caller-owned buffers.
  * llattn_args mirrors attn::Args (engine/attn.cu:51-64) field for field. */

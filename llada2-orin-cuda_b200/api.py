@@ -23,6 +23,8 @@ SCALE = 0.08838834764831845  # 1/sqrt(128), the constant engine/engine.cu:430 pa
 OK, EINVAL, ECUDA, ENOMEM, EDEVICE = 0, 1, 2, 3, 4
 IO_PRECISE_P = 1  # llattn_io.flags
 DENSE_STRIPS, DENSE_TILES, DENSE_TCGEN05 = 0, 1, 2
+F32, F16, BF16 = 0, 1, 2  # LLATTN_F32, ...
+MAX_AXES, MAX_ADAPTER_POOLS = 4, 4
 
 EXPORTS = (
     "llattn_version", "llattn_last_error", "llattn_pick_bpc", "llattn_chunks_for", "llattn_tile_units", "llattn_kv_commit",
@@ -31,6 +33,7 @@ EXPORTS = (
     "llattn_plan_update", "llattn_attention_host", "llattn_host_flush", "llattn_device_status",
     "llattn_dense_w4a8", "llattn_dense_preview", "llattn_dense_status", "llattn_dense_error_word", "llattn_kvpool_create", "llattn_kvpool_destroy", "llattn_kvpool_open", "llattn_kvpool_append", "llattn_kvpool_pages", "llattn_kvpool_mark_committed",
     "llattn_kvpool_close", "llattn_kvpool_stats", "llattn_attention_static", "llattn_wait_selftest",
+    "llattn_qk_norm_rope_axes", "llattn_qkv_prepare_commit_axes", "llattn_add_norm_q8", "llattn_adapters_w4a8",
 )
 
 
@@ -55,6 +58,11 @@ class _IO(Structure):
     _fields_ = [("Q", c_void_p), ("Kf", c_void_p), ("Vf", c_void_p), ("O16", c_void_p), ("O32", c_void_p),
                 ("LSE", c_void_p), ("q8", c_void_p), ("s8", c_void_p), ("sum8", c_void_p), ("scale", c_float),
                 ("flags", ctypes.c_uint32), ("cache_offset", c_int64)]
+
+
+class _AdapterPool(Structure):
+    _fields_ = [("A", c_void_p), ("B", c_void_p), ("scale", c_void_p), ("ranks", c_void_p), ("n", c_int32), ("rank", c_int32),
+                ("rows", c_int32), ("row0", c_int32), ("type", c_int32)]
 
 
 class PlanStats(Structure):
@@ -82,6 +90,14 @@ def lib() -> ctypes.CDLL:
                                           c_void_p, c_int, c_void_p]
         L.llattn_qkv_prepare_commit.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
                                                 c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]
+        L.llattn_qk_norm_rope_axes.argtypes = [c_void_p, c_void_p, c_int, ctypes.c_char_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
+                                               c_void_p, c_void_p, c_int, c_void_p]
+        L.llattn_qkv_prepare_commit_axes.argtypes = [c_void_p, c_void_p, c_int, ctypes.c_char_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
+                                                     c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]
+        L.llattn_add_norm_q8.argtypes = [c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_int, c_int, c_int, c_void_p]
+        L.llattn_adapters_w4a8.argtypes = [POINTER(_AdapterPool), c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p,
+                                           c_void_p, c_int, c_void_p]
         L.llattn_attn_partial.argtypes = [POINTER(_Args), c_int, c_void_p, c_void_p]
         L.llattn_attn_combine.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
                                           c_void_p, c_void_p, c_int, c_void_p]
@@ -131,6 +147,31 @@ def _ptr(t) -> Optional[int]:
     if not t.is_contiguous():
         raise ValueError("tensors crossing the C ABI must be contiguous")
     return t.data_ptr()
+
+
+def _types():
+    import torch
+    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+_TYPES = None
+
+
+def _type_of(t) -> int:
+    """LLATTN_F32, F16 or BF16 of a tensor (-1: none of them)."""
+    global _TYPES
+    if _TYPES is None:
+        _TYPES = _types()
+    return _TYPES.get(t.dtype, -1)
+
+
+def _here(*tensors) -> None:
+    """Every tensor (None: no tensor) is on the current device: the launch goes to that device, whatever the pointers."""
+    import torch
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
 
 
 _raw_stream = None
@@ -280,6 +321,146 @@ def qkv_prepare_commit(qkv, pos, gq, gk, eps, inv_freq_t, q, k, v, cache, max_bl
         raise ValueError("a prefill pass commits whole 32-token blocks")
     _check(lib().llattn_qkv_prepare_commit(_ptr(qkv), _ptr(pos), _ptr(gq), _ptr(gk), eps, _ptr(inv_freq_t), _ptr(q), _ptr(k),
                                            _ptr(v), T // BLK, _ptr(cache), _ptr(pages), max_blocks, blk, _stream(stream)))
+
+
+def rope_axes(sections, interleaved: bool = False) -> bytes:
+    """The axis of each of the 32 rotary frequencies, as qk_norm_rope_axes takes it: sections[a] of them belong to axis a - the first
+    sections[0] to axis 0, the next to axis 1, ..., or dealt to the axes in turn while an axis has some left (interleaved)."""
+    left = [int(n) for n in sections]
+    if not 1 <= len(left) <= MAX_AXES or min(left) < 0 or sum(left) != 32:
+        raise ValueError(f"1 to {MAX_AXES} sections that add up to 32, got {sections}")
+    if not interleaved:
+        return bytes(a for a, n in enumerate(left) for _ in range(n))
+    out = []
+    while len(out) < 32:
+        for a, n in enumerate(left):
+            if n:
+                left[a] -= 1
+                out.append(a)
+    return bytes(out)
+
+
+def _check_axes(qkv, pos, axis_of, gq, gk, inv_freq_t, q, k, v):
+    import torch
+    T = qkv.shape[0]
+    if qkv.shape != (T, (NQH + 2 * NKV) * D) or qkv.dtype != torch.float32 or pos.dim() != 2 or pos.shape[1] != T or pos.dtype != torch.int32:
+        raise ValueError("qkv is fp32 [T][3072], pos int32 [axes][T]")
+    if len(axis_of) != 32:
+        raise ValueError("axis_of has one axis for each of the 32 frequencies")
+    if any(t.numel() != n or t.dtype != torch.float32 for t, n in ((gq, D), (gk, D), (inv_freq_t, 32))):
+        raise ValueError("gq and gk are fp32 [128], inv_freq fp32 [32]")
+    if any(t.numel() != T * n * D or t.dtype != torch.float16 for t, n in ((q, NQH), (k, NKV), (v, NKV))):
+        raise ValueError("q is fp16 [T][16][128], k and v fp16 [T][4][128]")
+    return T
+
+
+def qk_norm_rope_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream=None) -> None:
+    """qk_norm_rope with several position axes: pos int32 [axes][T], axis_of the axis of each of the 32 frequencies (host; see rope_axes)."""
+    T = _check_axes(qkv, pos, axis_of, gq, gk, inv_freq_t, q, k, v)
+    _here(qkv, pos, gq, gk, inv_freq_t, q, k, v)
+    _check(lib().llattn_qk_norm_rope_axes(_ptr(qkv), _ptr(pos), pos.shape[0], bytes(axis_of), _ptr(gq), _ptr(gk), eps, _ptr(inv_freq_t), _ptr(q),
+                                          _ptr(k), _ptr(v), T, _stream(stream)))
+
+
+def qkv_prepare_commit_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, cache, max_blocks: int = 0, blk: int = 0, pages=None,
+                            stream=None) -> None:
+    """qkv_prepare_commit with several position axes, see qk_norm_rope_axes."""
+    T = _check_axes(qkv, pos, axis_of, gq, gk, inv_freq_t, q, k, v)
+    if T % BLK:
+        raise ValueError("a prefill pass commits whole 32-token blocks")
+    if pages is not None and pages.numel() != T // BLK * NKV:
+        raise ValueError("pages must hold nb * 4 indices")
+    _here(qkv, pos, gq, gk, inv_freq_t, q, k, v, cache, pages)
+    _check(lib().llattn_qkv_prepare_commit_axes(_ptr(qkv), _ptr(pos), pos.shape[0], bytes(axis_of), _ptr(gq), _ptr(gk), eps, _ptr(inv_freq_t),
+                                                _ptr(q), _ptr(k), _ptr(v), T // BLK, _ptr(cache), _ptr(pages), max_blocks, blk, _stream(stream)))
+
+
+# ------------------------------------------------------------------ norm, adapters
+
+def _rows(t, K: int, what: str):
+    """Data pointer and row distance of a matrix whose rows are contiguous."""
+    if t.dim() != 2 or t.shape[1] != K or (K > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: [T][{K}] with contiguous rows")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else K)
+
+
+def add_norm_q8(x, gain, eps, q=None, s=None, qsum=None, delta=None, y=None, stream=None) -> None:
+    """Residual addition, RMS norm and int8 activations in one pass (llattn_add_norm_q8). x fp32 [T][K] takes delta (fp32, fp16 or bf16 [T][K];
+    None: nothing is added and x is only read); q int8 [T][K] in fragment order, s fp32 and qsum int32 [T][K/128] are what dense_w4a8 and
+    adapters_w4a8 read; y fp16 or bf16 [T][K] the normalised values. The rows of x and delta may be further apart than K."""
+    import torch
+    T, K = x.shape
+    xp, ldx = _rows(x, K, "x")
+    dp, ldd = (None, 0) if delta is None else _rows(delta, K, "delta")
+    if x.dtype != torch.float32 or gain.dtype != torch.float32 or gain.numel() != K or (delta is not None and delta.shape[0] != T):
+        raise ValueError("x and gain are fp32, [T][K] and [K], delta [T][K]")
+    if q is not None and (q.shape != x.shape or q.dtype != torch.int8 or s is None or qsum is None or s.shape != (T, K // 128) or s.dtype != torch.float32 or
+                          qsum.shape != s.shape or qsum.dtype != torch.int32):
+        raise ValueError("q is int8 [T][K], s fp32 and qsum int32 [T][K / 128]")
+    if y is not None and y.shape != x.shape:
+        raise ValueError("y is [T][K]")
+    _here(x, gain, q, s, qsum, delta, y)
+    _check(lib().llattn_add_norm_q8(xp, ldx, dp, 0 if delta is None else _type_of(delta), ldd, _ptr(gain), eps, _ptr(q), _ptr(s), _ptr(qsum),
+                                    _ptr(y), 0 if y is None else _type_of(y), T, K, _stream(stream)))
+
+
+@dataclass
+class AdapterPool:
+    """The low-rank adapters of one part of a projection's output, rows [row0, row0 + rows): A [n][rank][K] and B [n][rows][rank], both fp16
+    or both bf16; scale fp32 [n] (None: 1); ranks int32 [n] (None: all have `rank`). Device tensors; their contents may be replaced at any time
+    between calls, a slot for one adapter after the other."""
+    A: object
+    B: object
+    row0: int = 0
+    scale: object = None
+    ranks: object = None
+
+    def _c(self) -> _AdapterPool:
+        import torch
+        A, B, n = self.A, self.B, self.A.shape[0]
+        if A.dim() != 3 or B.dim() != 3 or B.shape[0] != n or B.shape[2] != A.shape[1] or A.dtype != B.dtype:
+            raise ValueError("A is [n][rank][K], B [n][rows][rank], of one type")
+        if (self.scale is not None and (self.scale.numel() != n or self.scale.dtype != torch.float32)) or \
+           (self.ranks is not None and (self.ranks.numel() != n or self.ranks.dtype != torch.int32)):
+            raise ValueError("scale is fp32 [n], ranks int32 [n]")
+        return _AdapterPool(_ptr(A), _ptr(B), _ptr(self.scale), _ptr(self.ranks), n, A.shape[1], B.shape[1], self.row0, _type_of(A))
+
+
+class AdapterPools:
+    """One to four pools for calls of adapters_w4a8, checked once; holds their tensors."""
+
+    def __init__(self, pools: Sequence[AdapterPool]):
+        self.pools = list(pools)
+        if not self.pools or any(p.A.shape[2] != self.pools[0].A.shape[2] for p in self.pools):
+            raise ValueError("at least one pool, and one K for all")
+        self.K = self.pools[0].A.shape[2]
+        self.device = self.pools[0].A.get_device()
+        if any(t is not None and t.get_device() != self.device for p in self.pools for t in (p.A, p.B, p.scale, p.ranks)):
+            raise ValueError("the pools are on one device")
+        self._c = (_AdapterPool * len(self.pools))(*[p._c() for p in self.pools])
+
+
+def adapter_pools(pools: Sequence[AdapterPool]) -> AdapterPools:
+    return AdapterPools(pools)
+
+
+def adapters_w4a8(pools: AdapterPools, q, s, Y, seg_first, seg_adapter, stream=None) -> None:
+    """Adds the adapters of many requests to a projection's output Y (fp32 [ntokens][>= row0 + rows], rows contiguous), from the activations
+    (q int8 [ntokens][K] in fragment order, s fp32 [ntokens][K/128]) that dense_w4a8 reads (llattn_adapters_w4a8). Segment i is the tokens
+    seg_first[i] .. seg_first[i + 1] - 1 and has adapter seg_adapter[i] (-1: none); both are int32 device tensors."""
+    import torch
+    T, K = q.shape
+    yp, ldy = _rows(Y, Y.shape[-1], "Y")
+    nseg = seg_adapter.numel()
+    if K != pools.K or q.dtype != torch.int8 or s.shape != (T, K // 128) or s.dtype != torch.float32 or Y.shape[0] != T or Y.dtype != torch.float32:
+        raise ValueError(f"q is int8 [T][{pools.K}], s fp32 [T][{pools.K // 128}], Y fp32 [T][..]")
+    if seg_first.numel() != nseg + 1 or seg_first.dtype != torch.int32 or seg_adapter.dtype != torch.int32:
+        raise ValueError("seg_first is int32 [segments + 1], seg_adapter int32 [segments]")
+    if any(p.row0 + p.B.shape[1] > Y.shape[1] for p in pools.pools):
+        raise ValueError("a pool's rows reach beyond Y's")
+    _here(pools.pools[0].A, q, s, Y, seg_first, seg_adapter)
+    _check(lib().llattn_adapters_w4a8(pools._c, len(pools.pools), _ptr(q), _ptr(s), yp, ldy, T, K, _ptr(seg_first), _ptr(seg_adapter), nseg,
+                                      _stream(stream)))
 
 
 # ------------------------------------------------------------------ the reference operator pair

@@ -199,8 +199,8 @@ int llattn_kv_commit_paged(const void* Kf, const void* Vf, void* pool, const int
 
 namespace {
 int launch_prepare(const float* qkv, const int32_t* pos, const float* gq, const float* gk, float eps, const float* inv_freq,
-                   void* q, void* k, void* v, int T, void* records, const int32_t* pages, int max_blocks, int blk, void* stream) {
-    llattn::PrepArgs a{qkv, pos, gq, gk, inv_freq, eps, static_cast<half*>(q), static_cast<half*>(k), static_cast<half*>(v), T,
+                   void* q, void* k, void* v, int T, uint64_t axis_of, void* records, const int32_t* pages, int max_blocks, int blk, void* stream) {
+    llattn::PrepArgs a{qkv, pos, gq, gk, inv_freq, eps, static_cast<half*>(q), static_cast<half*>(k), static_cast<half*>(v), T, axis_of,
                        static_cast<uint8_t*>(records), pages, max_blocks, blk};
     const int blocks = (T + llattn::BLK - 1) / llattn::BLK;
     using namespace llattn;
@@ -214,25 +214,63 @@ int launch_prepare(const float* qkv, const int32_t* pos, const float* gq, const 
 }
 }  // namespace
 
+namespace {
+int prepare_only(const char* who, const float* qkv, const int32_t* pos, const float* gq, const float* gk, float eps, const float* inv_freq,
+                 void* q, void* k, void* v, int T, uint64_t axis_of, void* stream) {
+    if (!qkv || !pos || !gq || !gk || !inv_freq || !q || !k || !v) return fail(LLATTN_EINVAL, "%s: null pointer", who);
+    if (T < 0 || T > 1 << 24) return fail(LLATTN_EINVAL, "%s: T = %d", who, T);
+    if (!aligned16(k) || !aligned16(v)) return fail(LLATTN_EINVAL, "%s: k and v must be 16-byte aligned", who);
+    if (T == 0) return LLATTN_OK;
+    return launch_prepare(qkv, pos, gq, gk, eps, inv_freq, q, k, v, T, axis_of, nullptr, nullptr, 0, 0, stream);
+}
+int prepare_commit(const char* who, const float* qkv, const int32_t* pos, const float* gq, const float* gk, float eps, const float* inv_freq,
+                   void* q, void* k, void* v, int nb, uint64_t axis_of, void* cache, const int32_t* pages, int max_blocks, int blk, void* stream) {
+    if (!qkv || !pos || !gq || !gk || !inv_freq || !q || !k || !v || !cache) return fail(LLATTN_EINVAL, "%s: null pointer", who);
+    if (nb < 0 || nb > 65535) return fail(LLATTN_EINVAL, "%s: nb must be in [0, 65535]", who);
+    if (!pages && (blk < 0 || max_blocks <= 0 || blk + nb > max_blocks))
+        return fail(LLATTN_EINVAL, "%s: blocks [%d, %d) outside a cache of %d blocks", who, blk, blk + nb, max_blocks);
+    if (!aligned16(k) || !aligned16(v) || !aligned16(cache)) return fail(LLATTN_EINVAL, "%s: k, v and cache must be 16-byte aligned", who);
+    if (nb == 0) return LLATTN_OK;
+    return launch_prepare(qkv, pos, gq, gk, eps, inv_freq, q, k, v, nb * llattn::BLK, axis_of, cache, pages, max_blocks, blk, stream);
+}
+
+// The host array of 32 axes as two bits each.
+int pack_axes(const char* who, const uint8_t* axis_of, int naxes, uint64_t& packed) {
+    if (!axis_of) return fail(LLATTN_EINVAL, "%s: null pointer", who);
+    if (naxes < 1 || naxes > LLATTN_MAX_AXES) return fail(LLATTN_EINVAL, "%s: %d axes; 1 to %d", who, naxes, LLATTN_MAX_AXES);
+    packed = 0;
+    for (int i = 0; i < 32; ++i) {
+        if (axis_of[i] >= naxes) return fail(LLATTN_EINVAL, "%s: frequency %d is on axis %d of %d", who, i, int(axis_of[i]), naxes);
+        packed |= uint64_t(axis_of[i]) << (2 * i);
+    }
+    return LLATTN_OK;
+}
+}  // namespace
+
 int llattn_qk_norm_rope(const float* qkv, const int32_t* pos, const float* gq, const float* gk, float eps,
                         const float* inv_freq, void* q, void* k, void* v, int T, void* stream) {
-    if (!qkv || !pos || !gq || !gk || !inv_freq || !q || !k || !v) return fail(LLATTN_EINVAL, "qk_norm_rope: null pointer");
-    if (T < 0 || T > 1 << 24) return fail(LLATTN_EINVAL, "qk_norm_rope: T = %d", T);
-    if (!aligned16(k) || !aligned16(v)) return fail(LLATTN_EINVAL, "qk_norm_rope: k and v must be 16-byte aligned");
-    if (T == 0) return LLATTN_OK;
-    return launch_prepare(qkv, pos, gq, gk, eps, inv_freq, q, k, v, T, nullptr, nullptr, 0, 0, stream);
+    return prepare_only("qk_norm_rope", qkv, pos, gq, gk, eps, inv_freq, q, k, v, T, 0, stream);
 }
 
 int llattn_qkv_prepare_commit(const float* qkv, const int32_t* pos, const float* gq, const float* gk, float eps,
                               const float* inv_freq, void* q, void* k, void* v, int nb, void* cache, const int32_t* pages,
                               int max_blocks, int blk, void* stream) {
-    if (!qkv || !pos || !gq || !gk || !inv_freq || !q || !k || !v || !cache) return fail(LLATTN_EINVAL, "qkv_prepare_commit: null pointer");
-    if (nb < 0 || nb > 65535) return fail(LLATTN_EINVAL, "qkv_prepare_commit: nb must be in [0, 65535]");
-    if (!pages && (blk < 0 || max_blocks <= 0 || blk + nb > max_blocks))
-        return fail(LLATTN_EINVAL, "qkv_prepare_commit: blocks [%d, %d) outside a cache of %d blocks", blk, blk + nb, max_blocks);
-    if (!aligned16(k) || !aligned16(v) || !aligned16(cache)) return fail(LLATTN_EINVAL, "qkv_prepare_commit: k, v and cache must be 16-byte aligned");
-    if (nb == 0) return LLATTN_OK;
-    return launch_prepare(qkv, pos, gq, gk, eps, inv_freq, q, k, v, nb * llattn::BLK, cache, pages, max_blocks, blk, stream);
+    return prepare_commit("qkv_prepare_commit", qkv, pos, gq, gk, eps, inv_freq, q, k, v, nb, 0, cache, pages, max_blocks, blk, stream);
+}
+
+int llattn_qk_norm_rope_axes(const float* qkv, const int32_t* pos, int naxes, const uint8_t* axis_of, const float* gq, const float* gk, float eps,
+                             const float* inv_freq, void* q, void* k, void* v, int T, void* stream) {
+    uint64_t axes = 0;
+    if (int rc = pack_axes("qk_norm_rope_axes", axis_of, naxes, axes)) return rc;
+    return prepare_only("qk_norm_rope_axes", qkv, pos, gq, gk, eps, inv_freq, q, k, v, T, axes, stream);
+}
+
+int llattn_qkv_prepare_commit_axes(const float* qkv, const int32_t* pos, int naxes, const uint8_t* axis_of, const float* gq, const float* gk, float eps,
+                                   const float* inv_freq, void* q, void* k, void* v, int nb, void* cache, const int32_t* pages,
+                                   int max_blocks, int blk, void* stream) {
+    uint64_t axes = 0;
+    if (int rc = pack_axes("qkv_prepare_commit_axes", axis_of, naxes, axes)) return rc;
+    return prepare_commit("qkv_prepare_commit_axes", qkv, pos, gq, gk, eps, inv_freq, q, k, v, nb, axes, cache, pages, max_blocks, blk, stream);
 }
 
 // ------------------------------------------------------------------------------------------------------ consumer
@@ -406,6 +444,8 @@ int llattn_dense_status(void* stream, int* code) {
 
 #include "llattn_attention.inl"
 #include "kvpool.inl"
+#include "norm_q8.inl"
+#include "adapters.inl"
 
 // ====================================================================================================== no-allocation entry point
 // Scratch for llattn_attention_static: partial results (un-normalised O, reference maximum, row sum) of up to

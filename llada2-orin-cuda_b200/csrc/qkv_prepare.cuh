@@ -22,6 +22,9 @@
 // then share a lane and every global access of a warp is one contiguous segment. The float operations and their order
 // are the reference kernel's (sum of squares folded lane-wise then by a xor butterfly, rsqrtf, x*r*g, sincosf, one
 // fused multiply-add per rotated output), which is what makes the outputs bit-identical to it.
+//
+// Several position axes (time, height, width of an image's patch): a frequency belongs to one of up to four axes and its lane reads that axis's
+// position of the token. The rest is the same, so a token with one position on all axes gets the bits of the one-axis form.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,7 +39,7 @@ __host__ __device__ constexpr int prep_parts(int threads) { return BLK / (thread
 
 struct PrepArgs {
     const float* qkv;        // [T][3072]
-    const int* pos;          // [T]
+    const int* pos;          // [axes][T]
     const float* gq;         // [128]
     const float* gk;         // [128]
     const float* inv_freq;   // [32]
@@ -45,6 +48,7 @@ struct PrepArgs {
     half* k;                 // [T][4][128]
     half* v;                 // [T][4][128]
     int T;
+    uint64_t axis_of;        // two bits for each of the 32 frequencies: the axis whose position turns it
     // commit of the blocks this launch produces (records == nullptr: none). Block j of the launch, head h:
     // pages ? records + pages[j * 4 + h] * 4736 : records + (h * max_blocks + blk + j) * 4736
     uint8_t* records;
@@ -68,8 +72,8 @@ __device__ __forceinline__ void norm_rope_lane(float (&x)[4], const float* __res
     x[0] = lo; x[1] = hi;
 }
 
-__device__ __forceinline__ void rope_angle(const PrepArgs& a, int t, float freq, float& cs, float& sn) {
-    sincosf(float(a.pos[t]) * freq, &sn, &cs);
+__device__ __forceinline__ void rope_angle(const int* pos, int t, float freq, float& cs, float& sn) {
+    sincosf(float(pos[t]) * freq, &sn, &cs);
     cs = __bfloat162float(__float2bfloat16(cs));
     sn = __bfloat162float(__float2bfloat16(sn));
 }
@@ -80,6 +84,7 @@ __global__ void __launch_bounds__(NT) qkv_prepare_kernel(const PrepArgs a) {
     const int jb = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t0 = jb * BLK;
     const float freq = a.inv_freq[lane];
+    const int* pos = a.pos + size_t((a.axis_of >> (2 * lane)) & 3) * a.T;        // with one axis the same for all lanes
     if (!COMMIT || blockIdx.y >= NKV) {
         // ---- four heads of one token
         const int part = int(blockIdx.y) - (COMMIT ? NKV : 0), grp = part / prep_parts(NT), t = t0 + NT / 32 * (part % prep_parts(NT)) + warp;
@@ -93,7 +98,7 @@ __global__ void __launch_bounds__(NT) qkv_prepare_kernel(const PrepArgs a) {
         if (grp < 5) {
             const float* gain = grp < 4 ? a.gq : a.gk;
             float cs, sn;
-            rope_angle(a, t, freq, cs, sn);
+            rope_angle(pos, t, freq, cs, sn);
 #pragma unroll
             for (int h = 0; h < 4; ++h) norm_rope_lane(x[h], gain, lane, a.eps, cs, sn);
         }
@@ -120,7 +125,7 @@ __global__ void __launch_bounds__(NT) qkv_prepare_kernel(const PrepArgs a) {
         for (int k = 0; k < TOKS; ++k) {
             const int tok = TOKS * warp + k;
             float cs, sn;
-            rope_angle(a, t0 + tok, freq, cs, sn);
+            rope_angle(pos, t0 + tok, freq, cs, sn);
             norm_rope_lane(xk[k], a.gk, lane, a.eps, cs, sn);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
