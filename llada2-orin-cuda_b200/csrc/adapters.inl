@@ -75,17 +75,32 @@ __device__ __forceinline__ uint32_t to_tf32(float x) {
     return r;
 }
 
-// Shared memory of a CTA: where its tokens are, the partial sums of H by the half of the groups, H as value and remainder.
+// Shared memory of a CTA: where its tokens are, H as value and remainder, and the partial sums of H: a slot for each half of the groups of each CTA
+// of the cluster.
 template <int RT> struct AdapterSmem {
     static constexpr int R = 16 * RT, LDH = R + 2;          // a row of (value, remainder) pairs is 16 bytes longer than its values: conflict-free reads
-    int scan[AD_WARPS], tile[3];
-    float part[2][AD_TOK][R + 1];
+    static constexpr int LDP = AD_TOK + 8;                  // and eight rows of a slot are eight banks apart
+    int scan[AD_WARPS], tile[4];
     __align__(16) float2 h[AD_TOK][LDH];
+    float part[2][R][LDP];                                  // 2 x the cluster's CTAs of them
+    static constexpr int bytes(int ctas) { return int(sizeof(AdapterSmem)) + 2 * (ctas - 1) * R * LDP * 4; }
 };
+
+// The shared-memory address `addr` of this CTA in CTA `rank` of its cluster.
+__device__ __forceinline__ uint32_t cluster_address(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_store2(uint32_t addr, float a, float b) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // The segment and tokens of tile `want`, the tiles of the segments being counted through in order: {adapter or -1, first token, tokens}. Bounds that
 // are out of range or not in order give no tokens. Every thread calls.
-__device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, int (&scan)[AD_WARPS], int (&tile)[3]) {
+__device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, int (&scan)[AD_WARPS], int (&tile)[4]) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) { tile[0] = -1; tile[2] = 0; }
     int before = 0;
@@ -126,26 +141,45 @@ __device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, i
 }
 
 template <typename T, int RT>
-__global__ void __launch_bounds__(AD_THREADS) adapters_kernel(const __grid_constant__ AdapterParams p) {
+__global__ void __launch_bounds__(AD_THREADS, RT <= 4 ? 2 : 1) adapters_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(16) uint8_t ad_smem[];
-    AdapterSmem<RT>& sm = *reinterpret_cast<AdapterSmem<RT>*>(ad_smem);
+    using S = AdapterSmem<RT>;
+    S& sm = *reinterpret_cast<S*>(ad_smem);
     ptx::grid_dependency_wait();               // nothing is read or written before the kernel ahead has completed
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const AdapterPoolDesc& P = p.pool[blockIdx.y];
-    const int part = blockIdx.x % p.parts;
-    adapter_tile(p, blockIdx.x / p.parts, sm.scan, sm.tile);
+    const int parts = p.parts, part = blockIdx.x % parts;          // a cluster is the parts of one tile
+    if (parts > 1) cluster_arrive();           // the others may write here once this CTA is there
+    adapter_tile(p, blockIdx.x / parts, sm.scan, sm.tile);
     const int a = sm.tile[0], n0 = sm.tile[1], live = sm.tile[2];
-    if (live == 0 || a < 0 || a >= P.n) return;
-    const int rank = P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
-    if (rank == 0) return;
+    const int rank = live == 0 || a < 0 || a >= P.n ? 0 : P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
+    if (rank == 0) {                           // the same for the whole cluster
+        if (parts > 1) cluster_wait();
+        return;
+    }
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
     const int groups = p.K / DN_GROUP;
-    // ---- H, a warp for eight tokens and every second group
+    const int chunks = (P.rows + 31) / 32, per = (chunks + parts - 1) / parts, end = min(chunks, (part + 1) * per);
+    // ---- this warp's first 32 rows of Y are on their way from the start
+    float4 y[4][2];
+    auto load_y = [&](int c) {
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int n = 8 * nt + 2 * t + e, row = 32 * c + 4 * g;
+                if (n < live && row < P.rows) y[nt][e] = *reinterpret_cast<const float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row);
+            }
+    };
+    const int c0 = part * per + warp;
+    if (c0 < end) load_y(c0);
+    // ---- H over this CTA's groups (part, part + parts, ...), a warp for eight tokens and every second of them
     {
         const int nt = warp & 3, half_ = warp >> 2, n = 8 * nt + g;
         const uint16_t* A = static_cast<const uint16_t*>(P.A) + size_t(a) * P.rank * p.K + 4 * t;
         float h[RT][4] = {};
-        for (int gi = half_; gi < groups && 8 * nt < live; gi += 2) {
+#pragma unroll 1
+        for (int gi = part + half_ * parts; gi < groups && 8 * nt < live; gi += 2 * parts) {
             uint4 w[2] = {};
             if (n < live) {
                 const uint4* src = reinterpret_cast<const uint4*>(p.q + size_t(n0 + n) * p.K + size_t(gi) * DN_GROUP + 32 * t);
@@ -155,45 +189,59 @@ __global__ void __launch_bounds__(AD_THREADS) adapters_kernel(const __grid_const
 #pragma unroll
             for (int e = 0; e < 2; ++e) sx[e] = __ldg(p.s + size_t(n0 + min(8 * nt + 2 * t + e, live - 1)) * groups + gi);
             const uint32_t words[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
-            uint32_t b[8][2];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) T::widen(words[k], b[k][0], b[k][1]);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 if (16 * rt >= rank) break;
                 float c[4] = {};
                 const bool lo = 16 * rt + g < rank, hi = 16 * rt + g + 8 < rank;      // rows behind the rank are not read
                 const uint16_t* r0 = A + size_t(16 * rt + g) * p.K + size_t(gi) * DN_GROUP;
+                uint2 x[8], z[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    uint2 x = {}, y = {};
-                    if (lo) x = __ldg(reinterpret_cast<const uint2*>(r0 + 16 * k));
-                    if (hi) y = __ldg(reinterpret_cast<const uint2*>(r0 + size_t(8) * p.K + 16 * k));
-                    T::mma(c, x.x, y.x, x.y, y.y, b[k][0], b[k][1]);
+                    x[k] = z[k] = make_uint2(0u, 0u);
+                    if (lo) x[k] = __ldg(reinterpret_cast<const uint2*>(r0 + 16 * k));
+                    if (hi) z[k] = __ldg(reinterpret_cast<const uint2*>(r0 + size_t(8) * p.K + 16 * k));
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    uint32_t b0, b1;
+                    T::widen(words[k], b0, b1);
+                    T::mma(c, x[k].x, z[k].x, x[k].y, z[k].y, b0, b1);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) h[rt][e] = fmaf(sx[e & 1], c[e], h[rt][e]);
             }
         }
+        // to every CTA of the cluster: its slot 2 part + half there
+        const uint32_t mine = ptx::smem_u32(&sm.part[0][0][0]) + uint32_t(((2 * part + half_) * S::R + g) * S::LDP + 8 * nt + 2 * t) * 4;
+        if (parts > 1) cluster_wait();
+        for (int k = 0; k < parts; ++k) {
+            const uint32_t at = parts > 1 ? cluster_address(mine, k) : mine;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sm.part[half_][8 * nt + 2 * t + (e & 1)][16 * rt + g + 8 * (e >> 1)] = h[rt][e];
+            for (int rt = 0; rt < RT; ++rt) {
+                cluster_store2(at + 16 * rt * S::LDP * 4, h[rt][0], h[rt][1]);
+                cluster_store2(at + (16 * rt + 8) * S::LDP * 4, h[rt][2], h[rt][3]);
+            }
+        }
     }
-    __syncthreads();
-    for (int i = tid; i < AD_TOK * 16 * RT; i += AD_THREADS) {
-        const int n = i / (16 * RT), j = i % (16 * RT);
-        const float v = scale * (sm.part[0][n][j] + sm.part[1][n][j]);
+    if (parts > 1) { cluster_arrive(); cluster_wait(); }
+    else __syncthreads();
+    for (int i = tid; i < AD_TOK * S::R; i += AD_THREADS) {
+        const int n = i & 31, j = i >> 5;
+        float v = 0.f;
+        for (int k = 0; k < 2 * parts; ++k) v += sm.part[0][k * S::R + j][n];
+        v *= scale;
         const float hi = __uint_as_float(to_tf32(v));
         sm.h[n][j] = make_float2(hi, __uint_as_float(to_tf32(v - hi)));
     }
     __syncthreads();
     // ---- Y, a warp for 32 rows
-    const int chunks = (P.rows + 31) / 32, per = (chunks + p.parts - 1) / p.parts;
     const uint16_t* B = static_cast<const uint16_t*>(P.B) + size_t(a) * P.rows * P.rank;
-    for (int c = part * per + warp; c < min(chunks, (part + 1) * per); c += AD_WARPS) {
+#pragma unroll 1
+    for (int c = c0; c < end; c += AD_WARPS) {
         const int row = 32 * c + 4 * g;
         const bool mine = row < P.rows;
+        if (c != c0) load_y(c);
         float acc[2][4][4] = {};
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -204,8 +252,8 @@ __global__ void __launch_bounds__(AD_THREADS) adapters_kernel(const __grid_const
             for (int i = 0; i < 4; ++i) {
                 uint2 v = {};
                 if (mine && j < rank) v = __ldg(reinterpret_cast<const uint2*>(B + size_t(row + i) * P.rank + j));
-                const float2 x = T::unpack(v.x), y = T::unpack(v.y);
-                w[i][0] = __float_as_uint(x.x); w[i][1] = __float_as_uint(x.y); w[i][2] = __float_as_uint(y.x); w[i][3] = __float_as_uint(y.y);
+                const float2 u = T::unpack(v.x), z = T::unpack(v.y);
+                w[i][0] = __float_as_uint(u.x); w[i][1] = __float_as_uint(u.y); w[i][2] = __float_as_uint(z.x); w[i][3] = __float_as_uint(z.y);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (j + e >= rank) w[i][e] = 0u;          // what lies behind the rank, whatever it is, does not count
@@ -231,10 +279,9 @@ __global__ void __launch_bounds__(AD_THREADS) adapters_kernel(const __grid_const
             for (int e = 0; e < 2; ++e) {
                 const int n = 8 * nt + 2 * t + e;
                 if (n >= live) continue;
-                float4* y = reinterpret_cast<float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row);
-                float4 v = *y;
+                float4 v = y[nt][e];
                 v.x += acc[0][nt][e]; v.y += acc[0][nt][2 + e]; v.z += acc[1][nt][e]; v.w += acc[1][nt][2 + e];
-                *y = v;
+                *reinterpret_cast<float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row) = v;
             }
     }
 }
@@ -243,19 +290,23 @@ __global__ void __launch_bounds__(AD_THREADS) adapters_kernel(const __grid_const
 
 namespace {
 template <typename T, int RT>
-int launch_adapters(const llattn::AdapterParams& p, int npools, long long tiles, cudaStream_t stream) {
-    const int smem = sizeof(llattn::AdapterSmem<RT>);
-    auto* kernel = llattn::adapters_kernel<T, RT>;
+int launch_adapters(llattn::AdapterParams& p, int npools, long long tiles, int sms, cudaStream_t stream) {
+    using namespace llattn;
+    // CTAs of a cluster: as many as it takes to fill the chip
+    p.parts = 1;
+    while (p.parts < 8 && p.parts * RT < 16 && 2 * p.parts * tiles * npools <= 4 * sms) p.parts *= 2;
+    const int smem = AdapterSmem<RT>::bytes(p.parts);
+    auto* kernel = adapters_kernel<T, RT>;
     if (smem > 48 * 1024) CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    CU(launch_dependent_smem(kernel, dim3(unsigned(tiles * p.parts), npools), llattn::AD_THREADS, smem, stream, p));
+    CU(launch_dependent_cluster(kernel, dim3(unsigned(tiles * p.parts), npools), AD_THREADS, smem, p.parts, stream, p));
     return LLATTN_OK;
 }
 template <typename T>
-int launch_adapters_rank(const llattn::AdapterParams& p, int npools, int rank, long long tiles, cudaStream_t stream) {
-    if (rank <= 16) return launch_adapters<T, 1>(p, npools, tiles, stream);
-    if (rank <= 32) return launch_adapters<T, 2>(p, npools, tiles, stream);
-    if (rank <= 64) return launch_adapters<T, 4>(p, npools, tiles, stream);
-    return launch_adapters<T, 8>(p, npools, tiles, stream);
+int launch_adapters_rank(llattn::AdapterParams& p, int npools, int rank, long long tiles, int sms, cudaStream_t stream) {
+    if (rank <= 16) return launch_adapters<T, 1>(p, npools, tiles, sms, stream);
+    if (rank <= 32) return launch_adapters<T, 2>(p, npools, tiles, sms, stream);
+    if (rank <= 64) return launch_adapters<T, 4>(p, npools, tiles, sms, stream);
+    return launch_adapters<T, 8>(p, npools, tiles, sms, stream);
 }
 }  // namespace
 
@@ -299,9 +350,11 @@ extern "C" int llattn_adapters_w4a8(const llattn_adapter_pool* pools, int npools
     if (ntokens == 0 || nseg == 0) return LLATTN_OK;
     p.q = q; p.s = s; p.Y = Y; p.first = seg_first; p.adapter = seg_adapter;
     p.ldy = ldy; p.ntokens = ntokens; p.K = K; p.nseg = nseg;
-    p.parts = 8;
+    int dev = 0, sms = 0;
+    CU(cudaGetDevice(&dev));
+    CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     // no more tiles than this, however the segments cut the tokens: each has at most one that is not full
     const long long tiles = std::min<long long>(ntokens, (ntokens + (AD_TOK - 1ll) * nseg) / AD_TOK);
-    return pools[0].type == LLATTN_F16 ? launch_adapters_rank<AdapterF16>(p, npools, rank, tiles, as_stream(stream))
-                                       : launch_adapters_rank<AdapterBF16>(p, npools, rank, tiles, as_stream(stream));
+    return pools[0].type == LLATTN_F16 ? launch_adapters_rank<AdapterF16>(p, npools, rank, tiles, sms, as_stream(stream))
+                                       : launch_adapters_rank<AdapterBF16>(p, npools, rank, tiles, sms, as_stream(stream));
 }

@@ -110,6 +110,22 @@ cudaError_t launch_dependent_smem(void (*kernel)(KArgs...), dim3 grid, int threa
     if (e != cudaSuccess) cudaGetLastError();  // reported here, not to whoever asks next
     return e;
 }
+// The same with `ctas` CTAs next to one another in x as a cluster.
+template <typename... KArgs>
+cudaError_t launch_dependent_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, int ctas, cudaStream_t stream, KArgs... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.stream = stream; cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctas > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) cudaGetLastError();
+    return e;
+}
 template <typename... KArgs>
 cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, int threads, cudaStream_t stream, KArgs... args) {
     return launch_dependent_smem(kernel, grid, threads, 0, stream, args...);
