@@ -15,7 +15,7 @@
 
 namespace llattn {
 
-constexpr int AD_TOK = 32, AD_THREADS = 256, AD_WARPS = 8, AD_MAX_POOLS = LLATTN_MAX_ADAPTER_POOLS, AD_MAX_RANK = 128;
+constexpr int AD_THREADS = 256, AD_WARPS = 8, AD_MAX_POOLS = LLATTN_MAX_ADAPTER_POOLS, AD_MAX_RANK = 128;
 
 struct AdapterPoolDesc {
     const void* A;            // [n][rank][K]
@@ -75,15 +75,23 @@ __device__ __forceinline__ uint32_t to_tf32(float x) {
     return r;
 }
 
-// Shared memory of a CTA: where its tokens are, H as value and remainder, and the partial sums of H: a slot for each half of the groups of each CTA
-// of the cluster.
-template <int RT> struct AdapterSmem {
-    static constexpr int R = 16 * RT, LDH = R + 2;          // a row of (value, remainder) pairs is 16 bytes longer than its values: conflict-free reads
-    static constexpr int LDP = AD_TOK + 8;                  // and eight rows of a slot are eight banks apart
-    int scan[AD_WARPS], tile[4];
-    __align__(16) float2 h[AD_TOK][LDH];
-    float part[2][R][LDP];                                  // 2 x the cluster's CTAs of them
-    static constexpr int bytes(int ctas) { return int(sizeof(AdapterSmem)) + 2 * (ctas - 1) * R * LDP * 4; }
+// A CTA of RT sixteens of ranks and NT eights of tokens: its warps' shares and its shared memory.
+template <int RT, int NT> struct AdapterTile {
+    static constexpr int R = 16 * RT, TOK = 8 * NT;
+    // First product: a warp takes RW x 4 tiles of (16 ranks, 8 tokens) and every WK-th run of sixteen values of a group
+    static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WN = NT / 4, WK = AD_WARPS / (WR * WN);
+    // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
+    static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : 3;
+    // Then, in the same place: the warps' sums by share of the group, [WK][R][LDP]; behind them a slot [R][TOK] for the sums of each CTA of the
+    // cluster; H as pairs (value, remainder), [TOK][LDH], over the former once they have been passed on, behind them where there is no cluster.
+    static constexpr int LDP = TOK + 8, PART = WK * R * LDP * 4, LDH = R + 2, H = TOK * LDH * 8, SLOT = R * TOK * 4, SLOTS_AT = PART > H ? PART : H;
+    static constexpr int HEAD = 64;
+    static constexpr int bytes(int ctas) {
+        const int after = ctas > 1 ? SLOTS_AT + ctas * SLOT : PART + H;
+        return HEAD + (STAGES * STAGE > after ? STAGES * STAGE : after);
+    }
+    static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : 4;        // CTAs of a cluster
+    static_assert(bytes(MOST) <= 227 * 1024, "shared memory of the largest cluster");
 };
 
 // The shared-memory address `addr` of this CTA in CTA `rank` of its cluster.
@@ -92,15 +100,16 @@ __device__ __forceinline__ uint32_t cluster_address(uint32_t addr, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void cluster_store2(uint32_t addr, float a, float b) {
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
+__device__ __forceinline__ void cluster_store4(uint32_t addr, const float4& v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // The segment and tokens of tile `want`, the tiles of the segments being counted through in order: {adapter or -1, first token, tokens}. Bounds that
 // are out of range or not in order give no tokens. Every thread calls.
-__device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, int (&scan)[AD_WARPS], int (&tile)[4]) {
+template <int TOK>
+__device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, int* scan, int* tile) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) { tile[0] = -1; tile[2] = 0; }
     int before = 0;
@@ -112,7 +121,7 @@ __device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, i
             t1 = min(max(__ldg(p.first + i + 1), 0), p.ntokens);
             a = __ldg(p.adapter + i);
         }
-        const int tiles = t1 > t0 ? (t1 - t0 + AD_TOK - 1) / AD_TOK : 0;
+        const int tiles = t1 > t0 ? (t1 - t0 + TOK - 1) / TOK : 0;
         int upto = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -131,8 +140,8 @@ __device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, i
         const int k = want - before - (upto - tiles);        // the segment's tile, if it is one of its own
         if (k >= 0 && k < tiles) {
             tile[0] = a;
-            tile[1] = t0 + AD_TOK * k;
-            tile[2] = min(AD_TOK, t1 - t0 - AD_TOK * k);
+            tile[1] = t0 + TOK * k;
+            tile[2] = min(TOK, t1 - t0 - TOK * k);
         }
         before += total;
         if (before > want) break;
@@ -140,108 +149,151 @@ __device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, i
     __syncthreads();
 }
 
-template <typename T, int RT>
-__global__ void __launch_bounds__(AD_THREADS, RT <= 4 ? 2 : 1) adapters_kernel(const __grid_constant__ AdapterParams p) {
+template <typename T, int RT, int NT>
+__global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(16) uint8_t ad_smem[];
-    using S = AdapterSmem<RT>;
-    S& sm = *reinterpret_cast<S*>(ad_smem);
+    using C = AdapterTile<RT, NT>;
     ptx::grid_dependency_wait();               // nothing is read or written before the kernel ahead has completed
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const AdapterPoolDesc& P = p.pool[blockIdx.y];
     const int parts = p.parts, part = blockIdx.x % parts;          // a cluster is the parts of one tile
-    if (parts > 1) cluster_arrive();           // the others may write here once this CTA is there
-    adapter_tile(p, blockIdx.x / parts, sm.scan, sm.tile);
-    const int a = sm.tile[0], n0 = sm.tile[1], live = sm.tile[2];
-    const int rank = live == 0 || a < 0 || a >= P.n ? 0 : P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
-    if (rank == 0) {                           // the same for the whole cluster
-        if (parts > 1) cluster_wait();
-        return;
-    }
+    int* head = reinterpret_cast<int*>(ad_smem);
+    adapter_tile<C::TOK>(p, blockIdx.x / parts, head, head + AD_WARPS);
+    const int a = head[AD_WARPS], n0 = head[AD_WARPS + 1], live = head[AD_WARPS + 2];
+    if (live == 0 || a < 0 || a >= P.n) return;                    // the same for the whole cluster
+    uint8_t* area = ad_smem + C::HEAD;
+    const uint32_t area_s = ptx::smem_u32(area);
+    const int groups = p.K / DN_GROUP, mygroups = part < groups ? (groups - part + parts - 1) / parts : 0;
+    // ---- the groups part, part + parts, ... of the tokens' codes and of A, a few of them ahead
+    const uint16_t* A = static_cast<const uint16_t*>(P.A) + size_t(a) * P.rank * p.K;
+    auto fetch = [&](int i) {                  // one commit per call, so groups count uniformly
+        if (i < mygroups) {
+            const uint32_t st = area_s + uint32_t(i % C::STAGES) * C::STAGE;
+            const size_t at = size_t(part + i * parts) * DN_GROUP;
+            for (int k = tid; k < C::TOK * 8; k += AD_THREADS)
+                cp_async16(st + C::Q + (k >> 3) * C::LDQ + 16 * (k & 7), p.q + size_t(n0 + min(k >> 3, live - 1)) * p.K + at + 16 * (k & 7), (k >> 3) < live);
+            for (int k = tid; k < C::R * 16; k += AD_THREADS)
+                cp_async16(st + (k >> 4) * C::LDA + 16 * (k & 15), A + size_t(min(k >> 4, P.rank - 1)) * p.K + at + 8 * (k & 15), (k >> 4) < P.rank);
+            if (tid < C::TOK) cp_async4(st + C::SX + 4 * tid, p.s + size_t(n0 + min(tid, live - 1)) * groups + part + i * parts, tid < live);
+        }
+        cp_async_commit();
+    };
+    for (int i = 0; i < C::STAGES - 1; ++i) fetch(i);
+    const int rank = P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
-    const int groups = p.K / DN_GROUP;
-    const int chunks = (P.rows + 31) / 32, per = (chunks + parts - 1) / parts, end = min(chunks, (part + 1) * per);
-    // ---- this warp's first 32 rows of Y are on their way from the start
-    float4 y[4][2];
-    auto load_y = [&](int c) {
+    // ---- this CTA's rows of Y and B are wanted when H is done: into L2
+    const int chunks = (P.rows + 31) / 32, per = (chunks + parts - 1) / parts, first = part * per, end = min(chunks, first + per);
+    const uint16_t* B = static_cast<const uint16_t*>(P.B) + size_t(a) * P.rows * P.rank;
+    const int lines = max(end - first, 0);
+    for (int k = tid; k < live * lines; k += AD_THREADS)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.Y + (long long)(n0 + k / lines) * p.ldy + P.row0 + 32 * (first + k % lines)));
+    for (int k = tid; k < lines * 32 * P.rank / 64; k += AD_THREADS)
+        if (32 * first * P.rank + 64 * k < P.rows * P.rank) asm volatile("prefetch.global.L2 [%0];" ::"l"(B + size_t(32) * first * P.rank + 64 * k));
+    // ---- sums of H over these groups
+    const int wr = warp % C::WR, wn = warp / C::WR % C::WN, wk = warp / (C::WR * C::WN);
+    float h[C::RW][4][4] = {};
+#pragma unroll 1
+    for (int i = 0; i < mygroups; ++i) {
+        cp_async_wait<C::STAGES - 2>();
+        __syncthreads();                       // group i is in for everybody; group i - 1 is done with, its stage can be refilled
+        fetch(i + C::STAGES - 1);
+        const uint8_t* st = area + (i % C::STAGES) * C::STAGE;
+        constexpr int KN = 8 / C::WK;          // runs of sixteen: KN wk .. KN wk + KN - 1
+        float c[C::RW][4][4] = {};
+        uint32_t w[4][KN];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+            const uint8_t* src = st + C::Q + (32 * wn + 8 * nt + g) * C::LDQ + 32 * t + 4 * KN * wk;
+            if constexpr (KN == 1) w[nt][0] = *reinterpret_cast<const uint32_t*>(src);
+            else if constexpr (KN == 2) *reinterpret_cast<uint2*>(w[nt]) = *reinterpret_cast<const uint2*>(src);
+            else
+#pragma unroll
+                for (int k = 0; k < KN; k += 4) *reinterpret_cast<uint4*>(&w[nt][k]) = *reinterpret_cast<const uint4*>(src + 4 * k);
+        }
+#pragma unroll
+        for (int k = 0; k < KN; ++k) {
+            uint2 x[C::RW], z[C::RW];
+#pragma unroll
+            for (int r = 0; r < C::RW; ++r) {
+                const uint8_t* src = st + (16 * (C::RW * wr + r) + g) * C::LDA + 32 * (KN * wk + k) + 8 * t;
+                x[r] = *reinterpret_cast<const uint2*>(src);
+                z[r] = *reinterpret_cast<const uint2*>(src + 8 * C::LDA);
+            }
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) {
+                uint32_t b0, b1;
+                T::widen(w[nt][k], b0, b1);
+#pragma unroll
+                for (int r = 0; r < C::RW; ++r) T::mma(c[r][nt], x[r].x, z[r].x, x[r].y, z[r].y, b0, b1);
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt) {
+            const float2 sx = *reinterpret_cast<const float2*>(st + C::SX + 4 * (32 * wn + 8 * nt + 2 * t));
+#pragma unroll
+            for (int r = 0; r < C::RW; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[r][nt][e] = fmaf(e & 1 ? sx.y : sx.x, c[r][nt][e], h[r][nt][e]);
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();                           // the stages are done with
+    if (parts > 1) cluster_arrive();           // and may be written over by the others when all are there
+    float* sums = reinterpret_cast<float*>(area);
+#pragma unroll
+    for (int r = 0; r < C::RW; ++r)
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<float2*>(sums + (wk * C::R + 16 * (C::RW * wr + r) + g + 8 * e) * C::LDP + 32 * wn + 8 * nt + 2 * t) = make_float2(h[r][nt][2 * e], h[r][nt][2 * e + 1]);
+    __syncthreads();
+    if (parts > 1) {                           // this CTA's sums to its slot in every CTA
+        cluster_wait();
+        for (int i = tid; i < C::R * C::TOK / 4; i += AD_THREADS) {
+            const int n = 4 * i % C::TOK, j = 4 * i / C::TOK;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < C::WK; ++k) {
+                const float4 u = *reinterpret_cast<const float4*>(sums + (k * C::R + j) * C::LDP + n);
+                v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+            }
+            const uint32_t to = area_s + C::SLOTS_AT + part * C::SLOT + 16 * i;
+            for (int k = 0; k < parts; ++k) cluster_store4(cluster_address(to, k), v);
+        }
+        cluster_arrive();
+        cluster_wait();
+    }
+    if (rank == 0) return;                     // the same for the whole cluster, and nothing of it is written any more
+    uint8_t* hs = area + (parts > 1 ? 0 : C::PART);
+    {
+        const float* slots = parts > 1 ? reinterpret_cast<const float*>(area + C::SLOTS_AT) : sums;
+        const int ns = parts > 1 ? parts : C::WK, ld = parts > 1 ? C::TOK : C::LDP;
+        for (int i = tid; i < C::TOK * C::R; i += AD_THREADS) {
+            const int n = i % C::TOK, j = i / C::TOK;
+            float v = 0.f;
+            for (int k = 0; k < ns; ++k) v += slots[(k * C::R + j) * ld + n];
+            v = j < rank ? v * scale : 0.f;    // what A has behind the rank, whatever it is, does not count
+            const float hi = __uint_as_float(to_tf32(v));
+            *reinterpret_cast<float2*>(hs + (n * C::LDH + j) * 8) = make_float2(hi, __uint_as_float(to_tf32(v - hi)));
+        }
+    }
+    __syncthreads();
+    // ---- Y, a warp for 32 rows and 32 tokens
+    const int nn = 32 * (warp % C::WN);
+    if (nn >= live) return;
+#pragma unroll 1
+    for (int c = first + warp / C::WN; c < end; c += AD_WARPS / C::WN) {
+        const int row = 32 * c + 4 * g;
+        const bool mine = row < P.rows;
+        float4 y[4][2];
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int n = 8 * nt + 2 * t + e, row = 32 * c + 4 * g;
-                if (n < live && row < P.rows) y[nt][e] = *reinterpret_cast<const float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row);
+                const int n = nn + 8 * nt + 2 * t + e;
+                if (n < live && mine) y[nt][e] = *reinterpret_cast<const float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row);
             }
-    };
-    const int c0 = part * per + warp;
-    if (c0 < end) load_y(c0);
-    // ---- H over this CTA's groups (part, part + parts, ...), a warp for eight tokens and every second of them
-    {
-        const int nt = warp & 3, half_ = warp >> 2, n = 8 * nt + g;
-        const uint16_t* A = static_cast<const uint16_t*>(P.A) + size_t(a) * P.rank * p.K + 4 * t;
-        float h[RT][4] = {};
-#pragma unroll 1
-        for (int gi = part + half_ * parts; gi < groups && 8 * nt < live; gi += 2 * parts) {
-            uint4 w[2] = {};
-            if (n < live) {
-                const uint4* src = reinterpret_cast<const uint4*>(p.q + size_t(n0 + n) * p.K + size_t(gi) * DN_GROUP + 32 * t);
-                w[0] = __ldg(src); w[1] = __ldg(src + 1);
-            }
-            float sx[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) sx[e] = __ldg(p.s + size_t(n0 + min(8 * nt + 2 * t + e, live - 1)) * groups + gi);
-            const uint32_t words[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                if (16 * rt >= rank) break;
-                float c[4] = {};
-                const bool lo = 16 * rt + g < rank, hi = 16 * rt + g + 8 < rank;      // rows behind the rank are not read
-                const uint16_t* r0 = A + size_t(16 * rt + g) * p.K + size_t(gi) * DN_GROUP;
-                uint2 x[8], z[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    x[k] = z[k] = make_uint2(0u, 0u);
-                    if (lo) x[k] = __ldg(reinterpret_cast<const uint2*>(r0 + 16 * k));
-                    if (hi) z[k] = __ldg(reinterpret_cast<const uint2*>(r0 + size_t(8) * p.K + 16 * k));
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    uint32_t b0, b1;
-                    T::widen(words[k], b0, b1);
-                    T::mma(c, x[k].x, z[k].x, x[k].y, z[k].y, b0, b1);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) h[rt][e] = fmaf(sx[e & 1], c[e], h[rt][e]);
-            }
-        }
-        // to every CTA of the cluster: its slot 2 part + half there
-        const uint32_t mine = ptx::smem_u32(&sm.part[0][0][0]) + uint32_t(((2 * part + half_) * S::R + g) * S::LDP + 8 * nt + 2 * t) * 4;
-        if (parts > 1) cluster_wait();
-        for (int k = 0; k < parts; ++k) {
-            const uint32_t at = parts > 1 ? cluster_address(mine, k) : mine;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                cluster_store2(at + 16 * rt * S::LDP * 4, h[rt][0], h[rt][1]);
-                cluster_store2(at + (16 * rt + 8) * S::LDP * 4, h[rt][2], h[rt][3]);
-            }
-        }
-    }
-    if (parts > 1) { cluster_arrive(); cluster_wait(); }
-    else __syncthreads();
-    for (int i = tid; i < AD_TOK * S::R; i += AD_THREADS) {
-        const int n = i & 31, j = i >> 5;
-        float v = 0.f;
-        for (int k = 0; k < 2 * parts; ++k) v += sm.part[0][k * S::R + j][n];
-        v *= scale;
-        const float hi = __uint_as_float(to_tf32(v));
-        sm.h[n][j] = make_float2(hi, __uint_as_float(to_tf32(v - hi)));
-    }
-    __syncthreads();
-    // ---- Y, a warp for 32 rows
-    const uint16_t* B = static_cast<const uint16_t*>(P.B) + size_t(a) * P.rows * P.rank;
-#pragma unroll 1
-    for (int c = c0; c < end; c += AD_WARPS) {
-        const int row = 32 * c + 4 * g;
-        const bool mine = row < P.rows;
-        if (c != c0) load_y(c);
         float acc[2][4][4] = {};
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -256,11 +308,12 @@ __global__ void __launch_bounds__(AD_THREADS, RT <= 4 ? 2 : 1) adapters_kernel(c
                 w[i][0] = __float_as_uint(u.x); w[i][1] = __float_as_uint(u.y); w[i][2] = __float_as_uint(z.x); w[i][3] = __float_as_uint(z.y);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (j + e >= rank) w[i][e] = 0u;          // what lies behind the rank, whatever it is, does not count
+                    if (j + e >= rank) w[i][e] = 0u;          // nor what B has there
             }
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt) {
-                const float4 u = *reinterpret_cast<const float4*>(&sm.h[8 * nt + g][j]), v = *reinterpret_cast<const float4*>(&sm.h[8 * nt + g][j + 2]);
+                const uint8_t* src = hs + ((nn + 8 * nt + g) * C::LDH + j) * 8;
+                const float4 u = *reinterpret_cast<const float4*>(src), v = *reinterpret_cast<const float4*>(src + 16);
                 const uint32_t hi[4] = {__float_as_uint(u.x), __float_as_uint(u.z), __float_as_uint(v.x), __float_as_uint(v.z)};
                 const uint32_t lo[4] = {__float_as_uint(u.y), __float_as_uint(u.w), __float_as_uint(v.y), __float_as_uint(v.w)};
 #pragma unroll
@@ -277,7 +330,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT <= 4 ? 2 : 1) adapters_kernel(c
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int n = 8 * nt + 2 * t + e;
+                const int n = nn + 8 * nt + 2 * t + e;
                 if (n >= live) continue;
                 float4 v = y[nt][e];
                 v.x += acc[0][nt][e]; v.y += acc[0][nt][2 + e]; v.z += acc[1][nt][e]; v.w += acc[1][nt][2 + e];
@@ -289,24 +342,48 @@ __global__ void __launch_bounds__(AD_THREADS, RT <= 4 ? 2 : 1) adapters_kernel(c
 }  // namespace llattn
 
 namespace {
-template <typename T, int RT>
-int launch_adapters(llattn::AdapterParams& p, int npools, long long tiles, int sms, cudaStream_t stream) {
+// Tokens of a tile and CTAs of a cluster, by the sizes alone (the segments are on the device).
+struct AdapterForm { int tok, parts; long long tiles; };
+AdapterForm adapter_form(long long ntokens, long long nseg, int npools, int rt, int sms) {
+    AdapterForm f{};
+    f.tok = rt >= 4 && ntokens >= 128 * nseg && ntokens * npools >= 1024 ? 64 : 32;
+    // no more tiles than this, however the segments cut the tokens: each has at most one that is not full
+    f.tiles = std::min(ntokens, (ntokens + (f.tok - 1) * nseg) / f.tok);
+    const long long full = std::max(std::min(nseg, ntokens), (ntokens + f.tok - 1) / f.tok);
+    f.parts = 1;
+    while (f.parts < (rt == 8 && f.tok == 64 ? llattn::AdapterTile<8, 8>::MOST : 8) && 2 * f.parts * full * npools <= (rt > 2 ? 2 : 4) * sms) f.parts *= 2;
+    return f;
+}
+
+template <typename T, int RT, int NT>
+int launch_adapters_tile(llattn::AdapterParams& p, int npools, const AdapterForm& f, cudaStream_t stream) {
     using namespace llattn;
-    // CTAs of a cluster: as many as it takes to fill the chip
-    p.parts = 1;
-    while (p.parts < 8 && p.parts * RT < 16 && 2 * p.parts * tiles * npools <= 4 * sms) p.parts *= 2;
-    const int smem = AdapterSmem<RT>::bytes(p.parts);
-    auto* kernel = adapters_kernel<T, RT>;
-    if (smem > 48 * 1024) CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    CU(launch_dependent_cluster(kernel, dim3(unsigned(tiles * p.parts), npools), AD_THREADS, smem, p.parts, stream, p));
+    static std::once_flag once[64];
+    auto* kernel = adapters_kernel<T, RT, NT>;
+    constexpr int most = AdapterTile<RT, NT>::bytes(AdapterTile<RT, NT>::MOST);
+    int dev = 0;
+    CU(cudaGetDevice(&dev));
+    if (most > 48 * 1024) {
+        if (dev < 0 || dev >= 64) CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        else std::call_once(once[dev], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most); });
+    }
+    p.parts = f.parts;
+    CU(launch_dependent_cluster(kernel, dim3(unsigned(f.tiles * f.parts), npools), AD_THREADS, AdapterTile<RT, NT>::bytes(f.parts), f.parts, stream, p));
     return LLATTN_OK;
 }
+template <typename T, int RT>
+int launch_adapters(llattn::AdapterParams& p, int npools, int sms, cudaStream_t stream) {
+    const AdapterForm f = adapter_form(p.ntokens, p.nseg, npools, RT, sms);
+    if constexpr (RT >= 4)
+        if (f.tok == 64) return launch_adapters_tile<T, RT, 8>(p, npools, f, stream);
+    return launch_adapters_tile<T, RT, 4>(p, npools, f, stream);
+}
 template <typename T>
-int launch_adapters_rank(llattn::AdapterParams& p, int npools, int rank, long long tiles, int sms, cudaStream_t stream) {
-    if (rank <= 16) return launch_adapters<T, 1>(p, npools, tiles, sms, stream);
-    if (rank <= 32) return launch_adapters<T, 2>(p, npools, tiles, sms, stream);
-    if (rank <= 64) return launch_adapters<T, 4>(p, npools, tiles, sms, stream);
-    return launch_adapters<T, 8>(p, npools, tiles, sms, stream);
+int launch_adapters_rank(llattn::AdapterParams& p, int npools, int rank, int sms, cudaStream_t stream) {
+    if (rank <= 16) return launch_adapters<T, 1>(p, npools, sms, stream);
+    if (rank <= 32) return launch_adapters<T, 2>(p, npools, sms, stream);
+    if (rank <= 64) return launch_adapters<T, 4>(p, npools, sms, stream);
+    return launch_adapters<T, 8>(p, npools, sms, stream);
 }
 }  // namespace
 
@@ -353,8 +430,6 @@ extern "C" int llattn_adapters_w4a8(const llattn_adapter_pool* pools, int npools
     int dev = 0, sms = 0;
     CU(cudaGetDevice(&dev));
     CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    // no more tiles than this, however the segments cut the tokens: each has at most one that is not full
-    const long long tiles = std::min<long long>(ntokens, (ntokens + (AD_TOK - 1ll) * nseg) / AD_TOK);
-    return pools[0].type == LLATTN_F16 ? launch_adapters_rank<AdapterF16>(p, npools, rank, tiles, sms, as_stream(stream))
-                                       : launch_adapters_rank<AdapterBF16>(p, npools, rank, tiles, sms, as_stream(stream));
+    return pools[0].type == LLATTN_F16 ? launch_adapters_rank<AdapterF16>(p, npools, rank, sms, as_stream(stream))
+                                       : launch_adapters_rank<AdapterBF16>(p, npools, rank, sms, as_stream(stream));
 }
