@@ -82,15 +82,12 @@ template <int RT, int NT> struct AdapterTile {
     static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WN = NT / 4, WK = AD_WARPS / (WR * WN);
     // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
     static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : 3;
-    // Then, in the same place: the warps' sums by share of the group, [WK][R][LDP]; behind them a slot [R][TOK] for the sums of each CTA of the
-    // cluster; H as pairs (value, remainder), [TOK][LDH], over the former once they have been passed on, behind them where there is no cluster.
-    static constexpr int LDP = TOK + 8, PART = WK * R * LDP * 4, LDH = R + 2, H = TOK * LDH * 8, SLOT = R * TOK * 4, SLOTS_AT = PART > H ? PART : H;
+    // Then, in the same place: the warps' sums by share of the group, [WK][R][LDP], and H as pairs (value, remainder), [TOK][LDH]. In front, where
+    // there is a cluster, a slot [R][TOK] for the sums of each of its CTAs.
+    static constexpr int LDP = TOK + 8, PART = WK * R * LDP * 4, LDH = R + 2, H = TOK * LDH * 8, SLOT = R * TOK * 4;
     static constexpr int HEAD = 64;
-    static constexpr int bytes(int ctas) {
-        const int after = ctas > 1 ? SLOTS_AT + ctas * SLOT : PART + H;
-        return HEAD + (STAGES * STAGE > after ? STAGES * STAGE : after);
-    }
-    static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : 4;        // CTAs of a cluster
+    static constexpr int bytes(int ctas) { return HEAD + (ctas > 1 ? ctas * SLOT : 0) + (STAGES * STAGE > PART + H ? STAGES * STAGE : PART + H); }
+    static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : bytes(4) <= 227 * 1024 ? 4 : 2;        // CTAs of a cluster
     static_assert(bytes(MOST) <= 227 * 1024, "shared memory of the largest cluster");
 };
 
@@ -100,53 +97,59 @@ __device__ __forceinline__ uint32_t cluster_address(uint32_t addr, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void cluster_store4(uint32_t addr, const float4& v) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+// 16 bytes into another CTA's shared memory, counted on the barrier `bar` there.
+__device__ __forceinline__ void cluster_store4(uint32_t addr, const float4& v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                 ::"r"(addr), "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+// Behind a wait for that barrier: what the other CTAs have stored is visible (the wait itself acquires for this CTA only).
+__device__ __forceinline__ void cluster_acquire(uint32_t bar) {
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], 0;\n\t}\n" ::"r"(bar) : "memory");
+}
+// (Nothing is handed over by it: the barrier's initialisation has its own fence.)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// The segment and tokens of tile `want`, the tiles of the segments being counted through in order: {adapter or -1, first token, tokens}. Bounds that
-// are out of range or not in order give no tokens. Every thread calls.
+// Where tile `want` is, the tiles of the segments being counted through in order: the segment's adapter, or -1, first token and tokens (0: there is no
+// such tile). Bounds that are out of range or not in order give no tokens. Every warp for itself, a lane for a run of neighbouring segments:
+// one load behind the launch, and no barrier.
+struct AdapterPlace { int adapter, n0, live; };
 template <int TOK>
-__device__ __forceinline__ void adapter_tile(const AdapterParams& p, int want, int* scan, int* tile) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) { tile[0] = -1; tile[2] = 0; }
-    int before = 0;
-    for (int base = 0; base < p.nseg; base += AD_THREADS) {
-        const int i = base + tid;
-        int t0 = 0, t1 = 0, a = -1;
-        if (i < p.nseg) {
-            t0 = min(max(__ldg(p.first + i), 0), p.ntokens);
-            t1 = min(max(__ldg(p.first + i + 1), 0), p.ntokens);
-            a = __ldg(p.adapter + i);
-        }
-        const int tiles = t1 > t0 ? (t1 - t0 + TOK - 1) / TOK : 0;
-        int upto = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        __syncthreads();                       // the former round's sums are read, and tile is set
-        if (lane == 31) scan[warp] = upto;
-        __syncthreads();
-        int total = 0;
-#pragma unroll
-        for (int k = 0; k < AD_WARPS; ++k) {
-            if (k < warp) upto += scan[k];
-            total += scan[k];
-        }
-        const int k = want - before - (upto - tiles);        // the segment's tile, if it is one of its own
-        if (k >= 0 && k < tiles) {
-            tile[0] = a;
-            tile[1] = t0 + TOK * k;
-            tile[2] = min(TOK, t1 - t0 - TOK * k);
-        }
-        before += total;
-        if (before > want) break;
+__device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, int want, int lane) {
+    const int per = (p.nseg + 31) / 32, s0 = min(lane * per, p.nseg), s1 = min(s0 + per, p.nseg);
+    auto bound = [&](int i) { return min(max(__ldg(p.first + i), 0), p.ntokens); };
+    auto tiles = [](int t0, int t1) { return t1 > t0 ? (t1 - t0 + TOK - 1) / TOK : 0; };
+    int mine = 0, t0 = bound(s0);
+    int a = s0 < s1 ? __ldg(p.adapter + s0) : -1;             // with up to 32 segments all there is to it
+    for (int i = s0, t = t0; i < s1; ++i) {
+        const int t1 = bound(i + 1);
+        mine += tiles(t, t1);
+        t = t1;
     }
-    __syncthreads();
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    int k = want - (upto - mine), live = 0;
+    const bool found = k >= 0 && k < mine;
+    if (found)
+        for (int i = s0; i < s1; ++i) {
+            const int t1 = bound(i + 1), n = tiles(t0, t1);
+            if (k < n) {
+                if (i > s0) a = __ldg(p.adapter + i);
+                live = min(TOK, t1 - t0 - TOK * k);
+                t0 += TOK * k;
+                break;
+            }
+            k -= n;
+            t0 = t1;
+        }
+    const unsigned who = __ballot_sync(0xffffffffu, found);
+    const int from = who ? __ffs(who) - 1 : 0;
+    AdapterPlace at{__shfl_sync(0xffffffffu, a, from), __shfl_sync(0xffffffffu, t0, from), __shfl_sync(0xffffffffu, live, from)};
+    return at;
 }
 
 template <typename T, int RT, int NT>
@@ -157,11 +160,22 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const AdapterPoolDesc& P = p.pool[blockIdx.y];
     const int parts = p.parts, part = blockIdx.x % parts;          // a cluster is the parts of one tile
-    int* head = reinterpret_cast<int*>(ad_smem);
-    adapter_tile<C::TOK>(p, blockIdx.x / parts, head, head + AD_WARPS);
-    const int a = head[AD_WARPS], n0 = head[AD_WARPS + 1], live = head[AD_WARPS + 2];
+    const AdapterPlace at_ = adapter_place<C::TOK>(p, blockIdx.x / parts, lane);
+    const int a = at_.adapter, n0 = at_.n0, live = at_.live;
     if (live == 0 || a < 0 || a >= P.n) return;                    // the same for the whole cluster
-    uint8_t* area = ad_smem + C::HEAD;
+    // ---- a barrier that counts the sums of the cluster's CTAs in; the others may use it once all are here
+    const uint32_t bar = ptx::smem_u32(ad_smem), slots_s = ptx::smem_u32(ad_smem + C::HEAD);
+    volatile int* abort_flag = reinterpret_cast<int*>(ad_smem + 8);
+    if (parts > 1) {
+        if (tid == 0) {
+            *abort_flag = 0;
+            ptx::mbar_init(bar, 1);
+            ptx::fence_mbar_init();
+            ptx::mbar_arrive_expect_tx(bar, parts * C::SLOT);
+        }
+        cluster_arrive();
+    }
+    uint8_t* area = ad_smem + C::HEAD + (parts > 1 ? parts * C::SLOT : 0);
     const uint32_t area_s = ptx::smem_u32(area);
     const int groups = p.K / DN_GROUP, mygroups = part < groups ? (groups - part + parts - 1) / parts : 0;
     // ---- the groups part, part + parts, ... of the tokens' codes and of A, a few of them ahead
@@ -181,14 +195,39 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
     for (int i = 0; i < C::STAGES - 1; ++i) fetch(i);
     const int rank = P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
-    // ---- this CTA's rows of Y and B are wanted when H is done: into L2
+    // ---- this CTA's rows of Y and B are wanted when H is done: a small rank's into registers, a larger one's into L2
     const int chunks = (P.rows + 31) / 32, per = (chunks + parts - 1) / parts, first = part * per, end = min(chunks, first + per);
     const uint16_t* B = static_cast<const uint16_t*>(P.B) + size_t(a) * P.rows * P.rank;
-    const int lines = max(end - first, 0);
-    for (int k = tid; k < live * lines; k += AD_THREADS)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.Y + (long long)(n0 + k / lines) * p.ldy + P.row0 + 32 * (first + k % lines)));
-    for (int k = tid; k < lines * 32 * P.rank / 64; k += AD_THREADS)
-        if (32 * first * P.rank + 64 * k < P.rows * P.rank) asm volatile("prefetch.global.L2 [%0];" ::"l"(B + size_t(32) * first * P.rank + 64 * k));
+    const int nn = 32 * (warp % C::WN);
+    constexpr bool EARLY = RT == 1;
+    float4 y[4][2];
+    uint2 braw[4];
+    auto load_y = [&](int c) {
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int n = nn + 8 * nt + 2 * t + e, row = 32 * c + 4 * g;
+                if (n < live && row < P.rows) y[nt][e] = *reinterpret_cast<const float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row);
+            }
+    };
+    auto load_b = [&](int c, int rt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 32 * c + 4 * g + i, j = 16 * rt + 4 * t;
+            braw[i] = make_uint2(0u, 0u);
+            if (row < P.rows && j < P.rank) braw[i] = __ldg(reinterpret_cast<const uint2*>(B + size_t(row) * P.rank + j));
+        }
+    };
+    const int c0 = first + warp / C::WN;
+    if constexpr (EARLY) {
+        if (c0 < end) { load_y(c0); load_b(c0, 0); }
+    } else {
+        for (int n = warp; n < live; n += AD_WARPS)
+            for (int k = first + lane; k < end; k += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + 32 * k));
+        const uint16_t* last = B + size_t(min(32 * end, P.rows)) * P.rank;
+        for (const uint16_t* q = B + size_t(32 * first) * P.rank + 64 * tid; q < last; q += 64 * AD_THREADS) asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+    }
     // ---- sums of H over these groups
     const int wr = warp % C::WR, wn = warp / C::WR % C::WN, wk = warp / (C::WR * C::WN);
     float h[C::RW][4][4] = {};
@@ -238,7 +277,6 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
     }
     cp_async_wait<0>();
     __syncthreads();                           // the stages are done with
-    if (parts > 1) cluster_arrive();           // and may be written over by the others when all are there
     float* sums = reinterpret_cast<float*>(area);
 #pragma unroll
     for (int r = 0; r < C::RW; ++r)
@@ -248,6 +286,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
             for (int e = 0; e < 2; ++e)
                 *reinterpret_cast<float2*>(sums + (wk * C::R + 16 * (C::RW * wr + r) + g + 8 * e) * C::LDP + 32 * wn + 8 * nt + 2 * t) = make_float2(h[r][nt][2 * e], h[r][nt][2 * e + 1]);
     __syncthreads();
+    bool ok = true;
     if (parts > 1) {                           // this CTA's sums to its slot in every CTA
         cluster_wait();
         for (int i = tid; i < C::R * C::TOK / 4; i += AD_THREADS) {
@@ -258,16 +297,14 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
                 const float4 u = *reinterpret_cast<const float4*>(sums + (k * C::R + j) * C::LDP + n);
                 v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
             }
-            const uint32_t to = area_s + C::SLOTS_AT + part * C::SLOT + 16 * i;
-            for (int k = 0; k < parts; ++k) cluster_store4(cluster_address(to, k), v);
+            for (int k = 0; k < parts; ++k) cluster_store4(cluster_address(slots_s + part * C::SLOT + 16 * i, k), v, cluster_address(bar, k));
         }
-        cluster_arrive();
-        cluster_wait();
+        ok = ptx::mbar_wait(bar, 0, abort_flag);
+        cluster_acquire(bar);
     }
-    if (rank == 0) return;                     // the same for the whole cluster, and nothing of it is written any more
-    uint8_t* hs = area + (parts > 1 ? 0 : C::PART);
+    uint8_t* hs = area + C::PART;
     {
-        const float* slots = parts > 1 ? reinterpret_cast<const float*>(area + C::SLOTS_AT) : sums;
+        const float* slots = parts > 1 ? reinterpret_cast<const float*>(ad_smem + C::HEAD) : sums;
         const int ns = parts > 1 ? parts : C::WK, ld = parts > 1 ? C::TOK : C::LDP;
         for (int i = tid; i < C::TOK * C::R; i += AD_THREADS) {
             const int n = i % C::TOK, j = i / C::TOK;
@@ -278,33 +315,32 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
             *reinterpret_cast<float2*>(hs + (n * C::LDH + j) * 8) = make_float2(hi, __uint_as_float(to_tf32(v - hi)));
         }
     }
-    __syncthreads();
+    if (!__syncthreads_and(ok)) {              // Y of this tile is left as it was by this CTA
+        if (tid == 0) {
+            atomicOr(&g_dense_err, ERR_WAIT_FOLD);
+            *abort_flag = 0;
+            ptx::mbar_wait(bar, 0, abort_flag);                    // stores that are still on their way here
+        }
+        __syncthreads();
+        return;
+    }
+    if (rank == 0 || nn >= live) return;
     // ---- Y, a warp for 32 rows and 32 tokens
-    const int nn = 32 * (warp % C::WN);
-    if (nn >= live) return;
 #pragma unroll 1
-    for (int c = first + warp / C::WN; c < end; c += AD_WARPS / C::WN) {
+    for (int c = c0; c < end; c += AD_WARPS / C::WN) {
         const int row = 32 * c + 4 * g;
         const bool mine = row < P.rows;
-        float4 y[4][2];
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int n = nn + 8 * nt + 2 * t + e;
-                if (n < live && mine) y[nt][e] = *reinterpret_cast<const float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row);
-            }
+        if (!EARLY || c != c0) load_y(c);
         float acc[2][4][4] = {};
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             if (16 * rt >= rank) break;
             const int j = 16 * rt + 4 * t;
+            if (!EARLY || c != c0) load_b(c, rt);
             uint32_t w[4][4];                  // [row][j]: exact in tf32
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uint2 v = {};
-                if (mine && j < rank) v = __ldg(reinterpret_cast<const uint2*>(B + size_t(row + i) * P.rank + j));
-                const float2 u = T::unpack(v.x), z = T::unpack(v.y);
+                const float2 u = T::unpack(braw[i].x), z = T::unpack(braw[i].y);
                 w[i][0] = __float_as_uint(u.x); w[i][1] = __float_as_uint(u.y); w[i][2] = __float_as_uint(z.x); w[i][3] = __float_as_uint(z.y);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -346,12 +382,14 @@ namespace {
 struct AdapterForm { int tok, parts; long long tiles; };
 AdapterForm adapter_form(long long ntokens, long long nseg, int npools, int rt, int sms) {
     AdapterForm f{};
+    using namespace llattn;
     f.tok = rt >= 4 && ntokens >= 128 * nseg && ntokens * npools >= 1024 ? 64 : 32;
     // no more tiles than this, however the segments cut the tokens: each has at most one that is not full
     f.tiles = std::min(ntokens, (ntokens + (f.tok - 1) * nseg) / f.tok);
     const long long full = std::max(std::min(nseg, ntokens), (ntokens + f.tok - 1) / f.tok);
+    const int most = rt < 8 ? (f.tok == 32 ? 8 : AdapterTile<4, 8>::MOST) : f.tok == 32 ? AdapterTile<8, 4>::MOST : AdapterTile<8, 8>::MOST;
     f.parts = 1;
-    while (f.parts < (rt == 8 && f.tok == 64 ? llattn::AdapterTile<8, 8>::MOST : 8) && 2 * f.parts * full * npools <= (rt > 2 ? 2 : 4) * sms) f.parts *= 2;
+    while (f.parts < most && 2 * f.parts * full * npools <= 2 * sms) f.parts *= 2;
     return f;
 }
 
@@ -394,7 +432,7 @@ extern "C" int llattn_adapters_w4a8(const llattn_adapter_pool* pools, int npools
     if (npools < 1 || npools > AD_MAX_POOLS) return fail(LLATTN_EINVAL, "adapters_w4a8: %d pools; 1 to %d", npools, AD_MAX_POOLS);
     if (ntokens < 0 || ntokens > 1 << 22) return fail(LLATTN_EINVAL, "adapters_w4a8: ntokens = %d", ntokens);
     if (K <= 0 || K % DN_GROUP || K > 1 << 20) return fail(LLATTN_EINVAL, "adapters_w4a8: K = %d (a multiple of 128)", K);
-    if (nseg < 0 || nseg > 1 << 20) return fail(LLATTN_EINVAL, "adapters_w4a8: nseg = %d", nseg);
+    if (nseg < 0 || nseg > 1 << 16) return fail(LLATTN_EINVAL, "adapters_w4a8: nseg = %d", nseg);
     if (ldy <= 0 || ldy % 4 || ldy > int64_t(1) << 32) return fail(LLATTN_EINVAL, "adapters_w4a8: ldy = %lld (a multiple of 4)", (long long)ldy);
     if (!aligned16(q) || !aligned16(Y)) return fail(LLATTN_EINVAL, "adapters_w4a8: q and Y must be 16-byte aligned");
     if ((reinterpret_cast<uintptr_t>(s) | reinterpret_cast<uintptr_t>(seg_first) | reinterpret_cast<uintptr_t>(seg_adapter)) % 4)

@@ -169,7 +169,7 @@ def _args(api, **changed):
 
 @pytest.mark.parametrize("bad", [
     dict(none=True), dict(npools=0), dict(npools=5), dict(q=None), dict(s=None), dict(Y=None), dict(first=None), dict(adapter=None), dict(A=None), dict(B=None), dict(T=-1), dict(T=(1 << 22) + 1),
-    dict(K=0), dict(K=200), dict(K=(1 << 20) + 128), dict(nseg=-1), dict(nseg=(1 << 20) + 1), dict(ldy=0), dict(ldy=66), dict(ldy=60), dict(q=0x400008), dict(Y=0x600004), dict(s=0x500002), dict(first=0x700001),
+    dict(K=0), dict(K=200), dict(K=(1 << 20) + 128), dict(nseg=-1), dict(nseg=(1 << 16) + 1), dict(ldy=0), dict(ldy=66), dict(ldy=60), dict(q=0x400008), dict(Y=0x600004), dict(s=0x500002), dict(first=0x700001),
     dict(type=0), dict(type=3), dict(n=0), dict(rank=0), dict(rank=12), dict(rank=136), dict(rows=0), dict(rows=6), dict(rows=260), dict(row0=-4), dict(row0=2), dict(row0=196), dict(row0=2 ** 31 - 4),
     dict(A=0x100008), dict(B=0x200004), dict(scale=0x300002), dict(ranks=0x310001),
     dict(npools=2, pools=[{}, {}]), dict(npools=2, pools=[{}, dict(row0=60)]), dict(npools=2, pools=[{}, dict(row0=64, type=2)]), dict(npools=3, pools=[{}, dict(row0=128), dict(row0=100)]),
