@@ -69,6 +69,24 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// 32 ranks: four K-steps of kind::tf32 over 128-byte-swizzle tiles (A: 128 rows of B, B: the tokens' H). One elected lane issues.
+__device__ __forceinline__ void mma_tf32_block_warp(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate_first) {
+    asm volatile(
+        "{\n\t.reg .pred pe, pf, pt;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
+        "elect.sync _|pe, 0xffffffff;\n\t"
+        "setp.ne.b32 pf, %5, 0;\n\t setp.eq.b32 pt, 0, 0;\n\t"
+        "mov.b64 da, {%1, %3};\n\t mov.b64 db, {%2, %3};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, pf;\n\t"
+        "add.u32 x, %1, 2;\n\t add.u32 y, %2, 2;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, pt;\n\t"
+        "add.u32 x, %1, 4;\n\t add.u32 y, %2, 4;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, pt;\n\t"
+        "add.u32 x, %1, 6;\n\t add.u32 y, %2, 6;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, pt;\n\t"
+        "}\n" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate_first) : "memory");
+}
+// kind::tf32 instruction descriptor: fp32 accumulator, both operands tf32 and K-major.
+__host__ __device__ constexpr uint32_t idesc_tf32(int M, int N) { return (1u << 4) | (2u << 7) | (2u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24); }
 __device__ __forceinline__ uint32_t to_tf32(float x) {
     uint32_t r;
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
@@ -81,12 +99,17 @@ template <int RT, int NT> struct AdapterTile {
     // First product: a warp takes RW x 4 tiles of (16 ranks, 8 tokens) and every WK-th run of sixteen values of a group
     static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WN = NT / 4, WK = AD_WARPS / (WR * WN);
     // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
-    static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : 3;
-    // Then, in the same place: the warps' sums by share of the group, [WK][R][LDP], and H as pairs (value, remainder), [TOK][LDH]. In front, where
-    // there is a cluster, a slot [R][TOK] for the sums of each of its CTAs.
-    static constexpr int LDP = TOK + 8, PART = WK * R * LDP * 4, LDH = R + 2, H = TOK * LDH * 8, SLOT = R * TOK * 4;
-    static constexpr int HEAD = 64;
-    static constexpr int bytes(int ctas) { return HEAD + (ctas > 1 ? ctas * SLOT : 0) + (STAGES * STAGE > PART + H ? STAGES * STAGE : PART + H); }
+    static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 || NT > 4 ? 2 : RT > 1 ? 3 : 5;
+    // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], or the tensor cores' tile of B, and H: for few ranks as pairs
+    // (value, remainder), [TOK][LDH], else as the tensor cores' tiles of both. In front of all, where there is a cluster, a slot [TOK][R] for the sums of
+    // each of its CTAs.
+    static constexpr bool WIDE = RT >= 4;
+    static constexpr int LDP = R + 4, LDH = R + 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
+    static constexpr int WBLOCK = 128 * 128, HBLOCK = TOK * 128, HPART = R / 32 * HBLOCK;       // 32 ranks of 128 rows, of the tokens; all of them
+    static constexpr int H_AT = !WIDE ? SUMS : (SUMS > R / 32 * WBLOCK ? (SUMS + 1023) / 1024 * 1024 : R / 32 * WBLOCK);
+    static constexpr int AREA = H_AT + (WIDE ? 2 * HPART : TOK * LDH * 8);
+    static constexpr int HEAD = WIDE ? 1024 : 64;
+    static constexpr int bytes(int ctas) { return HEAD + (ctas > 1 ? ctas * SLOT : 0) + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
     static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : bytes(4) <= 227 * 1024 ? 4 : 2;        // CTAs of a cluster
     static_assert(bytes(MOST) <= 227 * 1024, "shared memory of the largest cluster");
 };
@@ -154,27 +177,30 @@ __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, in
 
 template <typename T, int RT, int NT>
 __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_kernel(const __grid_constant__ AdapterParams p) {
-    extern __shared__ __align__(16) uint8_t ad_smem[];
+    extern __shared__ __align__(1024) uint8_t ad_smem[];
     using C = AdapterTile<RT, NT>;
     ptx::grid_dependency_wait();               // nothing is read or written before the kernel ahead has completed
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const AdapterPoolDesc& P = p.pool[blockIdx.y];
     const int parts = p.parts, part = blockIdx.x % parts;          // a cluster is the parts of one tile
-    const AdapterPlace at_ = adapter_place<C::TOK>(p, blockIdx.x / parts, lane);
-    const int a = at_.adapter, n0 = at_.n0, live = at_.live;
+    const AdapterPlace place = adapter_place<C::TOK>(p, blockIdx.x / parts, lane);
+    const int a = place.adapter, n0 = place.n0, live = place.live;
     if (live == 0 || a < 0 || a >= P.n) return;                    // the same for the whole cluster
-    // ---- a barrier that counts the sums of the cluster's CTAs in; the others may use it once all are here
-    const uint32_t bar = ptx::smem_u32(ad_smem), slots_s = ptx::smem_u32(ad_smem + C::HEAD);
-    volatile int* abort_flag = reinterpret_cast<int*>(ad_smem + 8);
-    if (parts > 1) {
-        if (tid == 0) {
-            *abort_flag = 0;
-            ptx::mbar_init(bar, 1);
-            ptx::fence_mbar_init();
-            ptx::mbar_arrive_expect_tx(bar, parts * C::SLOT);
-        }
-        cluster_arrive();
+    if (C::WIDE && ptx::smem_u32(ad_smem) & 1023) {                // the tensor cores' tiles would lie elsewhere than they say
+        if (tid == 0) atomicOr(&g_dense_err, ERR_SMEM_ALIGN);
+        return;
     }
+    // ---- barriers: one counts the sums of the cluster's CTAs in (they may use it once all are here), one the tensor cores' products
+    const uint32_t bar = ptx::smem_u32(ad_smem), slots_s = ptx::smem_u32(ad_smem + C::HEAD);
+    volatile int* abort_flag = reinterpret_cast<int*>(ad_smem + 16);
+    if (tid == 0) {
+        *abort_flag = 0;
+        ptx::mbar_init(bar, 1);
+        ptx::mbar_init(bar + 8, 1);
+        ptx::fence_mbar_init();
+        if (parts > 1) ptx::mbar_arrive_expect_tx(bar, parts * C::SLOT);
+    }
+    if (parts > 1) cluster_arrive();
     uint8_t* area = ad_smem + C::HEAD + (parts > 1 ? parts * C::SLOT : 0);
     const uint32_t area_s = ptx::smem_u32(area);
     const int groups = p.K / DN_GROUP, mygroups = part < groups ? (groups - part + parts - 1) / parts : 0;
@@ -193,10 +219,13 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
         cp_async_commit();
     };
     for (int i = 0; i < C::STAGES - 1; ++i) fetch(i);
+    if constexpr (C::WIDE)
+        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), C::TOK); ptx::tmem_relinquish(); }
     const int rank = P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
-    // ---- this CTA's rows of Y and B are wanted when H is done: a small rank's into registers, a larger one's into L2
-    const int chunks = (P.rows + 31) / 32, per = (chunks + parts - 1) / parts, first = part * per, end = min(chunks, first + per);
+    // ---- this CTA's rows of Y and B are wanted when H is done: a small rank's first ones into registers, the others into L2
+    constexpr int ROWS = C::WIDE ? 128 : 32;   // of a step of the second product
+    const int steps = (P.rows + ROWS - 1) / ROWS, per = (steps + parts - 1) / parts, first = part * per, end = min(steps, first + per);
     const uint16_t* B = static_cast<const uint16_t*>(P.B) + size_t(a) * P.rows * P.rank;
     const int nn = 32 * (warp % C::WN);
     constexpr bool EARLY = RT == 1;
@@ -220,13 +249,13 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
         }
     };
     const int c0 = first + warp / C::WN;
-    if constexpr (EARLY) {
+    if constexpr (EARLY)
         if (c0 < end) { load_y(c0); load_b(c0, 0); }
-    } else {
+    {
+        const int from = ROWS * (EARLY ? min(first + AD_WARPS / C::WN, end) : first), to = min(ROWS * end, P.rows);
         for (int n = warp; n < live; n += AD_WARPS)
-            for (int k = first + lane; k < end; k += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + 32 * k));
-        const uint16_t* last = B + size_t(min(32 * end, P.rows)) * P.rank;
-        for (const uint16_t* q = B + size_t(32 * first) * P.rank + 64 * tid; q < last; q += 64 * AD_THREADS) asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+            for (int k = from + 32 * lane; k < to; k += 32 * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + k));
+        for (const uint16_t* q = B + size_t(from) * P.rank + 64 * tid; q < B + size_t(to) * P.rank; q += 64 * AD_THREADS) asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
     }
     // ---- sums of H over these groups
     const int wr = warp % C::WR, wn = warp / C::WR % C::WN, wk = warp / (C::WR * C::WN);
@@ -283,18 +312,18 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                *reinterpret_cast<float2*>(sums + (wk * C::R + 16 * (C::RW * wr + r) + g + 8 * e) * C::LDP + 32 * wn + 8 * nt + 2 * t) = make_float2(h[r][nt][2 * e], h[r][nt][2 * e + 1]);
+            for (int e = 0; e < 4; ++e)
+                sums[(wk * C::TOK + 32 * wn + 8 * nt + 2 * t + (e & 1)) * C::LDP + 16 * (C::RW * wr + r) + g + 8 * (e >> 1)] = h[r][nt][e];
     __syncthreads();
     bool ok = true;
     if (parts > 1) {                           // this CTA's sums to its slot in every CTA
         cluster_wait();
         for (int i = tid; i < C::R * C::TOK / 4; i += AD_THREADS) {
-            const int n = 4 * i % C::TOK, j = 4 * i / C::TOK;
+            const int n = 4 * i / C::R, j = 4 * i % C::R;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < C::WK; ++k) {
-                const float4 u = *reinterpret_cast<const float4*>(sums + (k * C::R + j) * C::LDP + n);
+                const float4 u = *reinterpret_cast<const float4*>(sums + (k * C::TOK + n) * C::LDP + j);
                 v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
             }
             for (int k = 0; k < parts; ++k) cluster_store4(cluster_address(slots_s + part * C::SLOT + 16 * i, k), v, cluster_address(bar, k));
@@ -302,76 +331,184 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
         ok = ptx::mbar_wait(bar, 0, abort_flag);
         cluster_acquire(bar);
     }
-    uint8_t* hs = area + C::PART;
+    uint8_t* hs = area + C::H_AT;
     {
         const float* slots = parts > 1 ? reinterpret_cast<const float*>(ad_smem + C::HEAD) : sums;
-        const int ns = parts > 1 ? parts : C::WK, ld = parts > 1 ? C::TOK : C::LDP;
-        for (int i = tid; i < C::TOK * C::R; i += AD_THREADS) {
-            const int n = i % C::TOK, j = i / C::TOK;
-            float v = 0.f;
-            for (int k = 0; k < ns; ++k) v += slots[(k * C::R + j) * ld + n];
-            v = j < rank ? v * scale : 0.f;    // what A has behind the rank, whatever it is, does not count
-            const float hi = __uint_as_float(to_tf32(v));
-            *reinterpret_cast<float2*>(hs + (n * C::LDH + j) * 8) = make_float2(hi, __uint_as_float(to_tf32(v - hi)));
+        const int ns = parts > 1 ? parts : C::WK, ld = parts > 1 ? C::R : C::LDP;
+        for (int i = tid; i < C::TOK * C::R / 4; i += AD_THREADS) {
+            const int n = 4 * i / C::R, j = 4 * i % C::R;
+            float v[4] = {};
+#pragma unroll 4
+            for (int k = 0; k < ns; ++k) {
+                const float4 u = *reinterpret_cast<const float4*>(slots + (k * C::TOK + n) * ld + j);
+                v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
+            }
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = j + e < rank ? v[e] * scale : 0.f;             // what A has behind the rank, whatever it is, does not count
+                hi[e] = to_tf32(x);
+                lo[e] = to_tf32(x - __uint_as_float(hi[e]));
+            }
+            if constexpr (C::WIDE) {
+                uint8_t* to = hs + j / 32 * C::HBLOCK + n * 128 + ((j % 32 / 4 ^ (n & 7)) << 4);
+                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(to + C::HPART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            } else {
+                uint4* to = reinterpret_cast<uint4*>(hs + (n * C::LDH + j) * 8);
+                to[0] = make_uint4(hi[0], lo[0], hi[1], lo[1]);
+                to[1] = make_uint4(hi[2], lo[2], hi[3], lo[3]);
+            }
         }
     }
-    if (!__syncthreads_and(ok)) {              // Y of this tile is left as it was by this CTA
-        if (tid == 0) {
+    ok = __syncthreads_and(ok);                // H is there; where sums are missing this CTA leaves Y as it is
+    if constexpr (C::WIDE) {
+        // ---- Y, 128 rows at a time on tcgen05: B as tf32 into its tile, both parts of H times it into tensor memory, from there a thread to a row
+        ptx::tc_fence_after();
+        const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 20), wtile = area_s;
+        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = idesc_tf32(128, C::TOK);
+        constexpr int CH = C::R / 8, LOADS = 128 * CH / AD_THREADS, HALF = C::TOK / 2;
+        uint4 wr16[LOADS];
+        auto load_w = [&](int c) {
+#pragma unroll
+            for (int m = 0; m < LOADS; ++m) {
+                const int k = tid + m * AD_THREADS, row = 128 * c + k / CH, j = k % CH * 8;
+                wr16[m] = make_uint4(0u, 0u, 0u, 0u);
+                if (c < end && row < P.rows && j < rank) wr16[m] = __ldg(reinterpret_cast<const uint4*>(B + size_t(row) * P.rank + j));
+            }
+        };
+        if (rank == 0) ok = false;
+        const bool wanted = rank != 0;
+        int issued = 0;
+        if (ok) load_w(first);
+#pragma unroll 1
+        for (int c = first; c < end; ++c) {
+            const int row = 128 * c + 32 * (warp & 3) + lane, nw = HALF * (warp >> 2);
+            float yv[HALF];
+            float* yrow = p.Y + (long long)(n0 + nw) * p.ldy + P.row0 + row;
+            if (ok && row < P.rows)
+#pragma unroll
+                for (int i = 0; i < HALF; ++i)
+                    if (nw + i < live) yv[i] = yrow[i * p.ldy];
+            if (ok) {
+#pragma unroll
+                for (int m = 0; m < LOADS; ++m) {
+                    const int k = tid + m * AD_THREADS, r = k / CH, j = k % CH * 8;
+                    const uint32_t raw[4] = {wr16[m].x, wr16[m].y, wr16[m].z, wr16[m].w};
+                    float f[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { const float2 u = T::unpack(raw[e]); f[2 * e] = u.x; f[2 * e + 1] = u.y; }
+                    if (j + 8 > rank)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (j + e >= rank) f[e] = 0.f;                     // nor what B has there
+                    uint8_t* to = area + j / 32 * C::WBLOCK + r * 128;
+                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 ^ (r & 7)) << 4)) = make_float4(f[0], f[1], f[2], f[3]);
+                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 + 1 ^ (r & 7)) << 4)) = make_float4(f[4], f[5], f[6], f[7]);
+                }
+                ptx::fence_proxy_async_smem();
+                ptx::tc_fence_before();
+            }
+            ok = __syncthreads_and(ok);        // B is there, the former rows have been read from tensor memory
+            if (!ok) break;
+            ptx::tc_fence_after();
+            ++issued;
+            if (warp == 0) {
+#pragma unroll 1
+                for (int k = 0; 32 * k < rank; ++k) {
+                    const uint32_t wa = ptx::desc_lo(wtile + k * C::WBLOCK, 16), ha = ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16);
+                    mma_tf32_block_warp(tmem, wa, ha + C::HPART / 16, dhi, idesc, k > 0);
+                    mma_tf32_block_warp(tmem, wa, ha, dhi, idesc, 1);
+                }
+                ptx::mma_commit_warp(bar + 8);
+            }
+            load_w(c + 1);
+            ok = ptx::mbar_wait_warp(bar + 8, (c - first) & 1, abort_flag);
+            ptx::tc_fence_after();
+            uint32_t acc[HALF];
+            const uint32_t from = tmem + (uint32_t(32 * (warp & 3)) << 16) + nw;
+            if constexpr (HALF == 32) ptx::tmem_ld32(from, acc);
+            else ptx::tmem_ld16(from, acc);
+            ptx::tmem_wait_ld_tied(acc);
+            ptx::tc_fence_before();
+            if (ok && row < P.rows)
+#pragma unroll
+                for (int i = 0; i < HALF; ++i)
+                    if (nw + i < live) yrow[i * p.ldy] = yv[i] + __uint_as_float(acc[i]);
+        }
+        ok = __syncthreads_and(ok);
+        if (tid == 0 && !ok && wanted) {
             atomicOr(&g_dense_err, ERR_WAIT_FOLD);
             *abort_flag = 0;
-            ptx::mbar_wait(bar, 0, abort_flag);                    // stores that are still on their way here
+            if (parts > 1) ptx::mbar_wait(bar, 0, abort_flag);                 // stores and products that are still on their way
+            *abort_flag = 0;
+            if (issued) ptx::mbar_wait(bar + 8, (issued - 1) & 1, abort_flag);
         }
         __syncthreads();
-        return;
-    }
-    if (rank == 0 || nn >= live) return;
-    // ---- Y, a warp for 32 rows and 32 tokens
-#pragma unroll 1
-    for (int c = c0; c < end; c += AD_WARPS / C::WN) {
-        const int row = 32 * c + 4 * g;
-        const bool mine = row < P.rows;
-        if (!EARLY || c != c0) load_y(c);
-        float acc[2][4][4] = {};
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (16 * rt >= rank) break;
-            const int j = 16 * rt + 4 * t;
-            if (!EARLY || c != c0) load_b(c, rt);
-            uint32_t w[4][4];                  // [row][j]: exact in tf32
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 u = T::unpack(braw[i].x), z = T::unpack(braw[i].y);
-                w[i][0] = __float_as_uint(u.x); w[i][1] = __float_as_uint(u.y); w[i][2] = __float_as_uint(z.x); w[i][3] = __float_as_uint(z.y);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (j + e >= rank) w[i][e] = 0u;          // nor what B has there
+        if (warp == 0) ptx::tmem_dealloc(tmem, C::TOK);
+    } else {
+        if (!ok) {
+            if (tid == 0) {
+                atomicOr(&g_dense_err, ERR_WAIT_FOLD);
+                *abort_flag = 0;
+                ptx::mbar_wait(bar, 0, abort_flag);                            // stores that are still on their way here
             }
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                const uint8_t* src = hs + ((nn + 8 * nt + g) * C::LDH + j) * 8;
-                const float4 u = *reinterpret_cast<const float4*>(src), v = *reinterpret_cast<const float4*>(src + 16);
-                const uint32_t hi[4] = {__float_as_uint(u.x), __float_as_uint(u.z), __float_as_uint(v.x), __float_as_uint(v.z)};
-                const uint32_t lo[4] = {__float_as_uint(u.y), __float_as_uint(u.w), __float_as_uint(v.y), __float_as_uint(v.w)};
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int k = 0; k < 4; k += 2) {
-                        mma_tf32(acc[i][nt], w[2 * i][k], w[2 * i + 1][k], w[2 * i][k + 1], w[2 * i + 1][k + 1], lo[k], lo[k + 1]);
-                        mma_tf32(acc[i][nt], w[2 * i][k], w[2 * i + 1][k], w[2 * i][k + 1], w[2 * i + 1][k + 1], hi[k], hi[k + 1]);
-                    }
-            }
+            __syncthreads();
+            return;
         }
-        if (!mine) continue;
+        if (rank == 0 || nn >= live) return;
+        // ---- Y, a warp for 32 rows and 32 tokens
+#pragma unroll 1
+        for (int c = c0; c < end; c += AD_WARPS / C::WN) {
+            const int row = 32 * c + 4 * g;
+            const bool mine = row < P.rows;
+            if (!EARLY || c != c0) load_y(c);
+            if (RT > 1 ? c == c0 : c != c0) load_b(c, 0);      // of the ranks that follow, and of the next rows, they are loaded one step ahead
+            float acc[2][4][4] = {};
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+            for (int rt = 0; rt < RT; ++rt) {
+                if (16 * rt >= rank) break;
+                const int j = 16 * rt + 4 * t;
+                uint32_t w[4][4];              // [row][j]: exact in tf32
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int n = nn + 8 * nt + 2 * t + e;
-                if (n >= live) continue;
-                float4 v = y[nt][e];
-                v.x += acc[0][nt][e]; v.y += acc[0][nt][2 + e]; v.z += acc[1][nt][e]; v.w += acc[1][nt][2 + e];
-                *reinterpret_cast<float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row) = v;
+                for (int i = 0; i < 4; ++i) {
+                    const float2 u = T::unpack(braw[i].x), z = T::unpack(braw[i].y);
+                    w[i][0] = __float_as_uint(u.x); w[i][1] = __float_as_uint(u.y); w[i][2] = __float_as_uint(z.x); w[i][3] = __float_as_uint(z.y);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (j + e >= rank) w[i][e] = 0u;       // nor what B has there
+                }
+                if constexpr (RT > 1) {
+                    if (16 * rt + 16 < rank) load_b(c, rt + 1);
+                    else load_b(c + AD_WARPS / C::WN, 0);      // (rows that P does not have are not read)
+                }
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt) {
+                    const uint8_t* src = hs + ((nn + 8 * nt + g) * C::LDH + j) * 8;
+                    const float4 u = *reinterpret_cast<const float4*>(src), v = *reinterpret_cast<const float4*>(src + 16);
+                    const uint32_t hi[4] = {__float_as_uint(u.x), __float_as_uint(u.z), __float_as_uint(v.x), __float_as_uint(v.z)};
+                    const uint32_t lo[4] = {__float_as_uint(u.y), __float_as_uint(u.w), __float_as_uint(v.y), __float_as_uint(v.w)};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int k = 0; k < 4; k += 2) {
+                            mma_tf32(acc[i][nt], w[2 * i][k], w[2 * i + 1][k], w[2 * i][k + 1], w[2 * i + 1][k + 1], lo[k], lo[k + 1]);
+                            mma_tf32(acc[i][nt], w[2 * i][k], w[2 * i + 1][k], w[2 * i][k + 1], w[2 * i + 1][k + 1], hi[k], hi[k + 1]);
+                        }
+                }
             }
+            if (!mine) continue;
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int n = nn + 8 * nt + 2 * t + e;
+                    if (n >= live) continue;
+                    float4 v = y[nt][e];
+                    v.x += acc[0][nt][e]; v.y += acc[0][nt][2 + e]; v.z += acc[1][nt][e]; v.w += acc[1][nt][2 + e];
+                    *reinterpret_cast<float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row) = v;
+                }
+        }
     }
 }
 
