@@ -51,13 +51,14 @@ struct AdapterF16 {
     static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const half2*>(&w)); }
 };
 struct AdapterBF16 {
-    // through fp32 (2^23 + v + 128, exact), whose upper halves are the bf16 numbers: eight bits are enough for them
+    // a byte v behind 0x43 is the bf16 number 128 + (v & 127), and with its sign bit alone 128 or 256: their difference is v, exact
     static __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-        const uint32_t u = w ^ 0x80808080u;
-        uint32_t f[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = __float_as_uint(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + e)) - 8388736.f);
-        lo = __byte_perm(f[0], f[1], 0x7632); hi = __byte_perm(f[2], f[3], 0x7632);
+        const uint32_t p = __byte_perm(w, 0x43434343u, 0x4140), q = __byte_perm(w, 0x43434343u, 0x4342);
+        lo = minus(p & 0xff7fff7fu, p & 0xff80ff80u); hi = minus(q & 0xff7fff7fu, q & 0xff80ff80u);
+    }
+    static __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) {
+        const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&x);
     }
     static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -113,6 +114,17 @@ template <int RT, int NT> struct AdapterTile {
     static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : bytes(4) <= 227 * 1024 ? 4 : 2;        // CTAs of a cluster
     static_assert(bytes(MOST) <= 227 * 1024, "shared memory of the largest cluster");
 };
+
+// Four neighbouring values added in L2: Y need not come here. Every value of a call is added to once, so no order matters; an fp32 addition rounded to
+// nearest (numbers below 2^-126 count as zero).
+__device__ __forceinline__ void add_to4(float* y, float a, float b, float c, float d) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(y), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+// A run of bytes into L2, both multiples of 16.
+__device__ __forceinline__ void l2_prefetch(const void* p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 
 // The shared-memory address `addr` of this CTA in CTA `rank` of its cluster.
 __device__ __forceinline__ uint32_t cluster_address(uint32_t addr, int rank) {
@@ -176,7 +188,7 @@ __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, in
 }
 
 template <typename T, int RT, int NT>
-__global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_kernel(const __grid_constant__ AdapterParams p) {
+__global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 1) adapters_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(1024) uint8_t ad_smem[];
     using C = AdapterTile<RT, NT>;
     ptx::grid_dependency_wait();               // nothing is read or written before the kernel ahead has completed
@@ -206,15 +218,29 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
     const int groups = p.K / DN_GROUP, mygroups = part < groups ? (groups - part + parts - 1) / parts : 0;
     // ---- the groups part, part + parts, ... of the tokens' codes and of A, a few of them ahead
     const uint16_t* A = static_cast<const uint16_t*>(P.A) + size_t(a) * P.rank * p.K;
+    const int8_t* qsrc[NT / 4];
+#pragma unroll
+    for (int m = 0; m < NT / 4; ++m) qsrc[m] = p.q + size_t(n0 + min(32 * m + (tid >> 3), live - 1)) * p.K + part * DN_GROUP + 16 * (tid & 7);
+    const uint16_t* asrc = A + size_t(tid >> 4) * p.K + part * DN_GROUP + 8 * (tid & 15);
+    const float* ssrc = p.s + size_t(n0 + min(tid, live - 1)) * groups + part;
+    const uint32_t qdst = area_s + C::Q + (tid >> 3) * C::LDQ + 16 * (tid & 7), adst = area_s + (tid >> 4) * C::LDA + 16 * (tid & 15), sdst = area_s + C::SX + 4 * tid;
+    uint32_t fst = 0;                          // the stage that is filled next
     auto fetch = [&](int i) {                  // one commit per call, so groups count uniformly
         if (i < mygroups) {
-            const uint32_t st = area_s + uint32_t(i % C::STAGES) * C::STAGE;
-            const size_t at = size_t(part + i * parts) * DN_GROUP;
-            for (int k = tid; k < C::TOK * 8; k += AD_THREADS)
-                cp_async16(st + C::Q + (k >> 3) * C::LDQ + 16 * (k & 7), p.q + size_t(n0 + min(k >> 3, live - 1)) * p.K + at + 16 * (k & 7), (k >> 3) < live);
-            for (int k = tid; k < C::R * 16; k += AD_THREADS)
-                cp_async16(st + (k >> 4) * C::LDA + 16 * (k & 15), A + size_t(min(k >> 4, P.rank - 1)) * p.K + at + 8 * (k & 15), (k >> 4) < P.rank);
-            if (tid < C::TOK) cp_async4(st + C::SX + 4 * tid, p.s + size_t(n0 + min(tid, live - 1)) * groups + part + i * parts, tid < live);
+#pragma unroll
+            for (int m = 0; m < NT / 4; ++m) {
+                cp_async16(qdst + fst + 32 * m * C::LDQ, qsrc[m], 32 * m + (tid >> 3) < live);
+                qsrc[m] += parts * DN_GROUP;
+            }
+#pragma unroll
+            for (int m = 0; m < RT; ++m) {     // behind the pool's ranks: zeros
+                const bool there = 16 * m + (tid >> 4) < P.rank;
+                cp_async16(adst + fst + 16 * m * C::LDA, there ? asrc + size_t(16 * m) * p.K : A, there);
+            }
+            asrc += parts * DN_GROUP;
+            if (tid < C::TOK) cp_async4(sdst + fst, ssrc, tid < live);
+            ssrc += parts;
+            fst = fst + C::STAGE == C::STAGES * C::STAGE ? 0 : fst + C::STAGE;
         }
         cp_async_commit();
     };
@@ -223,23 +249,13 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
         if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), C::TOK); ptx::tmem_relinquish(); }
     const int rank = P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
-    // ---- this CTA's rows of Y and B are wanted when H is done: a small rank's first ones into registers, the others into L2
+    // ---- this CTA's rows of Y and B are wanted when H is done: into L2, and a small rank's first ones of B into registers
     constexpr int ROWS = C::WIDE ? 128 : 32;   // of a step of the second product
     const int steps = (P.rows + ROWS - 1) / ROWS, per = (steps + parts - 1) / parts, first = part * per, end = min(steps, first + per);
     const uint16_t* B = static_cast<const uint16_t*>(P.B) + size_t(a) * P.rows * P.rank;
     const int nn = 32 * (warp % C::WN);
     constexpr bool EARLY = RT == 1;
-    float4 y[4][2];
     uint2 braw[4];
-    auto load_y = [&](int c) {
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int n = nn + 8 * nt + 2 * t + e, row = 32 * c + 4 * g;
-                if (n < live && row < P.rows) y[nt][e] = *reinterpret_cast<const float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row);
-            }
-    };
     auto load_b = [&](int c, int rt) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -250,12 +266,13 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
     };
     const int c0 = first + warp / C::WN;
     if constexpr (EARLY)
-        if (c0 < end) { load_y(c0); load_b(c0, 0); }
+        if (c0 < end) load_b(c0, 0);
     {
-        const int from = ROWS * (EARLY ? min(first + AD_WARPS / C::WN, end) : first), to = min(ROWS * end, P.rows);
-        for (int n = warp; n < live; n += AD_WARPS)
-            for (int k = from + 32 * lane; k < to; k += 32 * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + k));
-        for (const uint16_t* q = B + size_t(from) * P.rank + 64 * tid; q < B + size_t(to) * P.rank; q += 64 * AD_THREADS) asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+        const int from = ROWS * first, to = min(ROWS * end, P.rows);
+        if (to > from) {
+            if (tid < live) l2_prefetch(p.Y + (long long)(n0 + tid) * p.ldy + P.row0 + from, (to - from) * 4);
+            if (tid == C::TOK) l2_prefetch(B + size_t(from) * P.rank, (to - from) * P.rank * 2);
+        }
     }
     // ---- sums of H over these groups
     const int wr = warp % C::WR, wn = warp / C::WR % C::WN, wk = warp / (C::WR * C::WN);
@@ -383,13 +400,6 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
         if (ok) load_w(first);
 #pragma unroll 1
         for (int c = first; c < end; ++c) {
-            const int row = 128 * c + 32 * (warp & 3) + lane, nw = HALF * (warp >> 2);
-            float yv[HALF];
-            float* yrow = p.Y + (long long)(n0 + nw) * p.ldy + P.row0 + row;
-            if (ok && row < P.rows)
-#pragma unroll
-                for (int i = 0; i < HALF; ++i)
-                    if (nw + i < live) yv[i] = yrow[i * p.ldy];
             if (ok) {
 #pragma unroll
                 for (int m = 0; m < LOADS; ++m) {
@@ -402,9 +412,10 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             if (j + e >= rank) f[e] = 0.f;                     // nor what B has there
-                    uint8_t* to = area + j / 32 * C::WBLOCK + r * 128;
-                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 ^ (r & 7)) << 4)) = make_float4(f[0], f[1], f[2], f[3]);
-                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 + 1 ^ (r & 7)) << 4)) = make_float4(f[4], f[5], f[6], f[7]);
+                    const int g8 = r / 4 % 8;      // row 4 g + i of 32 is the tile's g + 8 i: a thread then gets four neighbouring rows from tensor memory
+                    uint8_t* to = area + j / 32 * C::WBLOCK + (r / 32 * 32 + g8 + r % 4 * 8) * 128;
+                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 ^ g8) << 4)) = make_float4(f[0], f[1], f[2], f[3]);
+                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 + 1 ^ g8) << 4)) = make_float4(f[4], f[5], f[6], f[7]);
                 }
                 ptx::fence_proxy_async_smem();
                 ptx::tc_fence_before();
@@ -425,16 +436,25 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
             load_w(c + 1);
             ok = ptx::mbar_wait_warp(bar + 8, (c - first) & 1, abort_flag);
             ptx::tc_fence_after();
-            uint32_t acc[HALF];
+            // rows 4 g and + 1 in a, + 2 and + 3 in b; tokens 8 i + 2 t and + 1
+            uint32_t ra[HALF / 2], rb[HALF / 2];
+            const int nw = HALF * (warp >> 2), row = 128 * c + 32 * (warp & 3) + 4 * g;
             const uint32_t from = tmem + (uint32_t(32 * (warp & 3)) << 16) + nw;
-            if constexpr (HALF == 32) ptx::tmem_ld32(from, acc);
-            else ptx::tmem_ld16(from, acc);
-            ptx::tmem_wait_ld_tied(acc);
+            ptx::tmem_ld16x256_cols(from, ra);
+            ptx::tmem_ld16x256_cols(from + (16u << 16), rb);
+            ptx::tmem_wait_ld_tied(ra);
+            ptx::tmem_wait_ld_tied(rb);
             ptx::tc_fence_before();
+            float* yrow = p.Y + (n0 + nw) * p.ldy + P.row0 + row;
             if (ok && row < P.rows)
 #pragma unroll
-                for (int i = 0; i < HALF; ++i)
-                    if (nw + i < live) yrow[i * p.ldy] = yv[i] + __uint_as_float(acc[i]);
+                for (int i = 0; i < HALF / 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int n = 8 * i + 2 * t + e;
+                        if (nw + n < live)
+                            add_to4(yrow + n * p.ldy, __uint_as_float(ra[4 * i + e]), __uint_as_float(ra[4 * i + 2 + e]), __uint_as_float(rb[4 * i + e]), __uint_as_float(rb[4 * i + 2 + e]));
+                    }
         }
         ok = __syncthreads_and(ok);
         if (tid == 0 && !ok && wanted) {
@@ -462,7 +482,6 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
         for (int c = c0; c < end; c += AD_WARPS / C::WN) {
             const int row = 32 * c + 4 * g;
             const bool mine = row < P.rows;
-            if (!EARLY || c != c0) load_y(c);
             if (RT > 1 ? c == c0 : c != c0) load_b(c, 0);      // of the ranks that follow, and of the next rows, they are loaded one step ahead
             float acc[2][4][4] = {};
 #pragma unroll
@@ -498,15 +517,14 @@ __global__ void __launch_bounds__(AD_THREADS, RT * NT <= 32 ? 2 : 1) adapters_ke
                 }
             }
             if (!mine) continue;
+            float* yrow = p.Y + n0 * p.ldy + P.row0 + row;
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int n = nn + 8 * nt + 2 * t + e;
                     if (n >= live) continue;
-                    float4 v = y[nt][e];
-                    v.x += acc[0][nt][e]; v.y += acc[0][nt][2 + e]; v.z += acc[1][nt][e]; v.w += acc[1][nt][2 + e];
-                    *reinterpret_cast<float4*>(p.Y + (long long)(n0 + n) * p.ldy + P.row0 + row) = v;
+                    add_to4(yrow + n * p.ldy, acc[0][nt][e], acc[0][nt][2 + e], acc[1][nt][e], acc[1][nt][2 + e]);
                 }
         }
     }
