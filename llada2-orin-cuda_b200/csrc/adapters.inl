@@ -100,17 +100,17 @@ template <int RT, int NT> struct AdapterTile {
     // First product: a warp takes RW x 4 tiles of (16 ranks, 8 tokens) and every WK-th run of sixteen values of a group
     static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WN = NT / 4, WK = AD_WARPS / (WR * WN);
     // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
-    static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 || NT > 4 ? 2 : RT > 1 ? 3 : 5;
+    static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : RT > 1 ? 3 : 5;
     // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], or the tensor cores' tile of B, and H: for few ranks as pairs
-    // (value, remainder), [TOK][LDH], else as the tensor cores' tiles of both. In front of all, where there is a cluster, a slot [TOK][R] for the sums of
-    // each of its CTAs.
+    // (value, remainder), [TOK][LDH], else as the tensor cores' tiles of both. In front of all a slot [TOK][R] for the sums of each other CTA of
+    // the cluster.
     static constexpr bool WIDE = RT >= 4;
     static constexpr int LDP = R + 4, LDH = R + 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
     static constexpr int WBLOCK = 128 * 128, HBLOCK = TOK * 128, HPART = R / 32 * HBLOCK;       // 32 ranks of 128 rows, of the tokens; all of them
     static constexpr int H_AT = !WIDE ? SUMS : (SUMS > R / 32 * WBLOCK ? (SUMS + 1023) / 1024 * 1024 : R / 32 * WBLOCK);
     static constexpr int AREA = H_AT + (WIDE ? 2 * HPART : TOK * LDH * 8);
     static constexpr int HEAD = WIDE ? 1024 : 64;
-    static constexpr int bytes(int ctas) { return HEAD + (ctas > 1 ? ctas * SLOT : 0) + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
+    static constexpr int bytes(int ctas) { return HEAD + (ctas - 1) * SLOT + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
     static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : bytes(4) <= 227 * 1024 ? 4 : 2;        // CTAs of a cluster
     static_assert(bytes(MOST) <= 227 * 1024, "shared memory of the largest cluster");
 };
@@ -210,10 +210,10 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
         ptx::mbar_init(bar, 1);
         ptx::mbar_init(bar + 8, 1);
         ptx::fence_mbar_init();
-        if (parts > 1) ptx::mbar_arrive_expect_tx(bar, parts * C::SLOT);
+        if (parts > 1) ptx::mbar_arrive_expect_tx(bar, (parts - 1) * C::SLOT);
     }
     if (parts > 1) cluster_arrive();
-    uint8_t* area = ad_smem + C::HEAD + (parts > 1 ? parts * C::SLOT : 0);
+    uint8_t* area = ad_smem + C::HEAD + (parts - 1) * C::SLOT;
     const uint32_t area_s = ptx::smem_u32(area);
     const int groups = p.K / DN_GROUP, mygroups = part < groups ? (groups - part + parts - 1) / parts : 0;
     // ---- the groups part, part + parts, ... of the tokens' codes and of A, a few of them ahead
@@ -249,30 +249,27 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
         if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), C::TOK); ptx::tmem_relinquish(); }
     const int rank = P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
-    // ---- this CTA's rows of Y and B are wanted when H is done: into L2, and a small rank's first ones of B into registers
+    // ---- this CTA's rows of B are wanted when H is done: into L2, and a small rank's first ones into registers
     constexpr int ROWS = C::WIDE ? 128 : 32;   // of a step of the second product
     const int steps = (P.rows + ROWS - 1) / ROWS, per = (steps + parts - 1) / parts, first = part * per, end = min(steps, first + per);
     const uint16_t* B = static_cast<const uint16_t*>(P.B) + size_t(a) * P.rows * P.rank;
     const int nn = 32 * (warp % C::WN);
     constexpr bool EARLY = RT == 1;
     uint2 braw[4];
-    auto load_b = [&](int c, int rt) {
+    auto load_b = [&](uint2 (&to)[4], int c, int rt) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = 32 * c + 4 * g + i, j = 16 * rt + 4 * t;
-            braw[i] = make_uint2(0u, 0u);
-            if (row < P.rows && j < P.rank) braw[i] = __ldg(reinterpret_cast<const uint2*>(B + size_t(row) * P.rank + j));
+            to[i] = make_uint2(0u, 0u);
+            if (row < P.rows && j < P.rank) to[i] = __ldg(reinterpret_cast<const uint2*>(B + size_t(row) * P.rank + j));
         }
     };
     const int c0 = first + warp / C::WN;
     if constexpr (EARLY)
-        if (c0 < end) load_b(c0, 0);
+        if (c0 < end) load_b(braw, c0, 0);
     {
         const int from = ROWS * first, to = min(ROWS * end, P.rows);
-        if (to > from) {
-            if (tid < live) l2_prefetch(p.Y + (long long)(n0 + tid) * p.ldy + P.row0 + from, (to - from) * 4);
-            if (tid == C::TOK) l2_prefetch(B + size_t(from) * P.rank, (to - from) * P.rank * 2);
-        }
+        if (tid == 0 && to > from) l2_prefetch(B + size_t(from) * P.rank, (to - from) * P.rank * 2);
     }
     // ---- sums of H over these groups
     const int wr = warp % C::WR, wn = warp / C::WR % C::WN, wk = warp / (C::WR * C::WN);
@@ -332,32 +329,40 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
             for (int e = 0; e < 4; ++e)
                 sums[(wk * C::TOK + 32 * wn + 8 * nt + 2 * t + (e & 1)) * C::LDP + 16 * (C::RW * wr + r) + g + 8 * (e >> 1)] = h[r][nt][e];
     __syncthreads();
+    // ---- four ranks of a token at a time: this CTA's sums, to a slot in every other CTA of the cluster, and all CTAs' in their order
+    constexpr int QUADS = (C::R * C::TOK / 4 + AD_THREADS - 1) / AD_THREADS;
+    float4 own[QUADS];
     bool ok = true;
-    if (parts > 1) {                           // this CTA's sums to its slot in every CTA
-        cluster_wait();
-        for (int i = tid; i < C::R * C::TOK / 4; i += AD_THREADS) {
-            const int n = 4 * i / C::R, j = 4 * i % C::R;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (parts > 1) cluster_wait();
+#pragma unroll
+    for (int m = 0; m < QUADS; ++m) {
+        const int i = tid + m * AD_THREADS, n = 4 * i / C::R, j = 4 * i % C::R;
+        own[m] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (n < C::TOK) {
 #pragma unroll
             for (int k = 0; k < C::WK; ++k) {
                 const float4 u = *reinterpret_cast<const float4*>(sums + (k * C::TOK + n) * C::LDP + j);
-                v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+                own[m].x += u.x; own[m].y += u.y; own[m].z += u.z; own[m].w += u.w;
             }
-            for (int k = 0; k < parts; ++k) cluster_store4(cluster_address(slots_s + part * C::SLOT + 16 * i, k), v, cluster_address(bar, k));
+            for (int k = 0; k < parts; ++k)
+                if (k != part) cluster_store4(cluster_address(slots_s + (part - (part > k)) * C::SLOT + 16 * i, k), own[m], cluster_address(bar, k));
         }
+    }
+    if (parts > 1) {
         ok = ptx::mbar_wait(bar, 0, abort_flag);
         cluster_acquire(bar);
     }
     uint8_t* hs = area + C::H_AT;
     {
-        const float* slots = parts > 1 ? reinterpret_cast<const float*>(ad_smem + C::HEAD) : sums;
-        const int ns = parts > 1 ? parts : C::WK, ld = parts > 1 ? C::R : C::LDP;
-        for (int i = tid; i < C::TOK * C::R / 4; i += AD_THREADS) {
-            const int n = 4 * i / C::R, j = 4 * i % C::R;
+        const float4* slots = reinterpret_cast<const float4*>(ad_smem + C::HEAD);
+#pragma unroll
+        for (int m = 0; m < QUADS; ++m) {
+            const int i = tid + m * AD_THREADS, n = 4 * i / C::R, j = 4 * i % C::R;
+            if (n >= C::TOK) break;
             float v[4] = {};
 #pragma unroll 4
-            for (int k = 0; k < ns; ++k) {
-                const float4 u = *reinterpret_cast<const float4*>(slots + (k * C::TOK + n) * ld + j);
+            for (int k = 0; k < parts; ++k) {
+                const float4 u = k == part ? own[m] : slots[(k - (k > part)) * (C::SLOT / 16) + i];
                 v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
             }
             uint32_t hi[4], lo[4];
@@ -482,7 +487,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
         for (int c = c0; c < end; c += AD_WARPS / C::WN) {
             const int row = 32 * c + 4 * g;
             const bool mine = row < P.rows;
-            if (RT > 1 ? c == c0 : c != c0) load_b(c, 0);      // of the ranks that follow, and of the next rows, they are loaded one step ahead
+            if (!EARLY && c == c0) load_b(braw, c, 0);         // of the ranks that follow, and of the next rows, they are loaded one step ahead
             float acc[2][4][4] = {};
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -497,10 +502,8 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
                     for (int e = 0; e < 4; ++e)
                         if (j + e >= rank) w[i][e] = 0u;       // nor what B has there
                 }
-                if constexpr (RT > 1) {
-                    if (16 * rt + 16 < rank) load_b(c, rt + 1);
-                    else load_b(c + AD_WARPS / C::WN, 0);      // (rows that P does not have are not read)
-                }
+                const bool last = 16 * rt + 16 >= rank;
+                if (!last || c + AD_WARPS / C::WN < end) load_b(braw, last ? c + AD_WARPS / C::WN : c, last ? 0 : rt + 1);
 #pragma unroll
                 for (int nt = 0; nt < 4; ++nt) {
                     const uint8_t* src = hs + ((nn + 8 * nt + g) * C::LDH + j) * 8;
