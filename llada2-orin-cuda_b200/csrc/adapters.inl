@@ -15,7 +15,7 @@
 
 namespace llattn {
 
-constexpr int AD_THREADS = 256, AD_WARPS = 8, AD_MAX_POOLS = LLATTN_MAX_ADAPTER_POOLS, AD_MAX_RANK = 128;
+constexpr int AD_TOK = 32, AD_THREADS = 256, AD_WARPS = 8, AD_MAX_POOLS = LLATTN_MAX_ADAPTER_POOLS, AD_MAX_RANK = 128;
 
 struct AdapterPoolDesc {
     const void* A;            // [n][rank][K]
@@ -94,11 +94,11 @@ __device__ __forceinline__ uint32_t to_tf32(float x) {
     return r;
 }
 
-// A CTA of RT sixteens of ranks and NT eights of tokens: its warps' shares and its shared memory.
-template <int RT, int NT> struct AdapterTile {
-    static constexpr int R = 16 * RT, TOK = 8 * NT;
+// A CTA of RT sixteens of ranks and 32 tokens: its warps' shares and its shared memory.
+template <int RT> struct AdapterTile {
+    static constexpr int R = 16 * RT, TOK = AD_TOK;
     // First product: a warp takes RW x 4 tiles of (16 ranks, 8 tokens) and every WK-th run of sixteen values of a group
-    static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WN = NT / 4, WK = AD_WARPS / (WR * WN);
+    static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WK = AD_WARPS / WR;
     // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
     static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : RT > 1 ? 3 : 5;
     // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], or the tensor cores' tile of B, and H: for few ranks as pairs
@@ -111,8 +111,6 @@ template <int RT, int NT> struct AdapterTile {
     static constexpr int AREA = H_AT + (WIDE ? 2 * HPART : TOK * LDH * 8);
     static constexpr int HEAD = WIDE ? 1024 : 64;
     static constexpr int bytes(int ctas) { return HEAD + (ctas - 1) * SLOT + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
-    static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : bytes(4) <= 227 * 1024 ? 4 : 2;        // CTAs of a cluster
-    static_assert(bytes(MOST) <= 227 * 1024, "shared memory of the largest cluster");
 };
 
 // Four neighbouring values added in L2: Y need not come here. Every value of a call is added to once, so no order matters; an fp32 addition rounded to
@@ -149,11 +147,10 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // such tile). Bounds that are out of range or not in order give no tokens. Every warp for itself, a lane for a run of neighbouring segments:
 // one load behind the launch, and no barrier.
 struct AdapterPlace { int adapter, n0, live; };
-template <int TOK>
 __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, int want, int lane) {
     const int per = (p.nseg + 31) / 32, s0 = min(lane * per, p.nseg), s1 = min(s0 + per, p.nseg);
     auto bound = [&](int i) { return min(max(__ldg(p.first + i), 0), p.ntokens); };
-    auto tiles = [](int t0, int t1) { return t1 > t0 ? (t1 - t0 + TOK - 1) / TOK : 0; };
+    auto tiles = [](int t0, int t1) { return t1 > t0 ? (t1 - t0 + AD_TOK - 1) / AD_TOK : 0; };
     int mine = 0, t0 = bound(s0);
     int a = s0 < s1 ? __ldg(p.adapter + s0) : -1;             // with up to 32 segments all there is to it
     for (int i = s0, t = t0; i < s1; ++i) {
@@ -174,8 +171,8 @@ __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, in
             const int t1 = bound(i + 1), n = tiles(t0, t1);
             if (k < n) {
                 if (i > s0) a = __ldg(p.adapter + i);
-                live = min(TOK, t1 - t0 - TOK * k);
-                t0 += TOK * k;
+                live = min(AD_TOK, t1 - t0 - AD_TOK * k);
+                t0 += AD_TOK * k;
                 break;
             }
             k -= n;
@@ -187,15 +184,15 @@ __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, in
     return at;
 }
 
-template <typename T, int RT, int NT>
-__global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 1) adapters_kernel(const __grid_constant__ AdapterParams p) {
+template <typename T, int RT>
+__global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(1024) uint8_t ad_smem[];
-    using C = AdapterTile<RT, NT>;
+    using C = AdapterTile<RT>;
     ptx::grid_dependency_wait();               // nothing is read or written before the kernel ahead has completed
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const AdapterPoolDesc& P = p.pool[blockIdx.y];
     const int parts = p.parts, part = blockIdx.x % parts;          // a cluster is the parts of one tile
-    const AdapterPlace place = adapter_place<C::TOK>(p, blockIdx.x / parts, lane);
+    const AdapterPlace place = adapter_place(p, blockIdx.x / parts, lane);
     const int a = place.adapter, n0 = place.n0, live = place.live;
     if (live == 0 || a < 0 || a >= P.n) return;                    // the same for the whole cluster
     if (C::WIDE && ptx::smem_u32(ad_smem) & 1023) {                // the tensor cores' tiles would lie elsewhere than they say
@@ -218,27 +215,22 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
     const int groups = p.K / DN_GROUP, mygroups = part < groups ? (groups - part + parts - 1) / parts : 0;
     // ---- the groups part, part + parts, ... of the tokens' codes and of A, a few of them ahead
     const uint16_t* A = static_cast<const uint16_t*>(P.A) + size_t(a) * P.rank * p.K;
-    const int8_t* qsrc[NT / 4];
-#pragma unroll
-    for (int m = 0; m < NT / 4; ++m) qsrc[m] = p.q + size_t(n0 + min(32 * m + (tid >> 3), live - 1)) * p.K + part * DN_GROUP + 16 * (tid & 7);
+    const int8_t* qsrc = p.q + size_t(n0 + min(tid >> 3, live - 1)) * p.K + part * DN_GROUP + 16 * (tid & 7);
     const uint16_t* asrc = A + size_t(tid >> 4) * p.K + part * DN_GROUP + 8 * (tid & 15);
     const float* ssrc = p.s + size_t(n0 + min(tid, live - 1)) * groups + part;
     const uint32_t qdst = area_s + C::Q + (tid >> 3) * C::LDQ + 16 * (tid & 7), adst = area_s + (tid >> 4) * C::LDA + 16 * (tid & 15), sdst = area_s + C::SX + 4 * tid;
     uint32_t fst = 0;                          // the stage that is filled next
     auto fetch = [&](int i) {                  // one commit per call, so groups count uniformly
         if (i < mygroups) {
-#pragma unroll
-            for (int m = 0; m < NT / 4; ++m) {
-                cp_async16(qdst + fst + 32 * m * C::LDQ, qsrc[m], 32 * m + (tid >> 3) < live);
-                qsrc[m] += parts * DN_GROUP;
-            }
+            cp_async16(qdst + fst, qsrc, (tid >> 3) < live);
+            qsrc += parts * DN_GROUP;
 #pragma unroll
             for (int m = 0; m < RT; ++m) {     // behind the pool's ranks: zeros
                 const bool there = 16 * m + (tid >> 4) < P.rank;
                 cp_async16(adst + fst + 16 * m * C::LDA, there ? asrc + size_t(16 * m) * p.K : A, there);
             }
             asrc += parts * DN_GROUP;
-            if (tid < C::TOK) cp_async4(sdst + fst, ssrc, tid < live);
+            if (tid < AD_TOK) cp_async4(sdst + fst, ssrc, tid < live);
             ssrc += parts;
             fst = fst + C::STAGE == C::STAGES * C::STAGE ? 0 : fst + C::STAGE;
         }
@@ -246,14 +238,13 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
     };
     for (int i = 0; i < C::STAGES - 1; ++i) fetch(i);
     if constexpr (C::WIDE)
-        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), C::TOK); ptx::tmem_relinquish(); }
-    const int rank = P.ranks ? min(max(__ldg(P.ranks + a), 0), P.rank) : P.rank;
+        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), AD_TOK); ptx::tmem_relinquish(); }
+    const int rank_there = P.ranks ? __ldg(P.ranks + a) : P.rank;  // looked at when the sums are there: a wait for it here would hold up what follows
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
     // ---- this CTA's rows of B are wanted when H is done: into L2, and a small rank's first ones into registers
     constexpr int ROWS = C::WIDE ? 128 : 32;   // of a step of the second product
     const int steps = (P.rows + ROWS - 1) / ROWS, per = (steps + parts - 1) / parts, first = part * per, end = min(steps, first + per);
     const uint16_t* B = static_cast<const uint16_t*>(P.B) + size_t(a) * P.rows * P.rank;
-    const int nn = 32 * (warp % C::WN);
     constexpr bool EARLY = RT == 1;
     uint2 braw[4];
     auto load_b = [&](uint2 (&to)[4], int c, int rt) {
@@ -264,7 +255,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
             if (row < P.rows && j < P.rank) to[i] = __ldg(reinterpret_cast<const uint2*>(B + size_t(row) * P.rank + j));
         }
     };
-    const int c0 = first + warp / C::WN;
+    const int c0 = first + warp;
     if constexpr (EARLY)
         if (c0 < end) load_b(braw, c0, 0);
     {
@@ -272,7 +263,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
         if (tid == 0 && to > from) l2_prefetch(B + size_t(from) * P.rank, (to - from) * P.rank * 2);
     }
     // ---- sums of H over these groups
-    const int wr = warp % C::WR, wn = warp / C::WR % C::WN, wk = warp / (C::WR * C::WN);
+    const int wr = warp % C::WR, wk = warp / C::WR;
     float h[C::RW][4][4] = {};
 #pragma unroll 1
     for (int i = 0; i < mygroups; ++i) {
@@ -285,7 +276,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
         uint32_t w[4][KN];
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
-            const uint8_t* src = st + C::Q + (32 * wn + 8 * nt + g) * C::LDQ + 32 * t + 4 * KN * wk;
+            const uint8_t* src = st + C::Q + (8 * nt + g) * C::LDQ + 32 * t + 4 * KN * wk;
             if constexpr (KN == 1) w[nt][0] = *reinterpret_cast<const uint32_t*>(src);
             else if constexpr (KN == 2) *reinterpret_cast<uint2*>(w[nt]) = *reinterpret_cast<const uint2*>(src);
             else
@@ -311,7 +302,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
         }
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
-            const float2 sx = *reinterpret_cast<const float2*>(st + C::SX + 4 * (32 * wn + 8 * nt + 2 * t));
+            const float2 sx = *reinterpret_cast<const float2*>(st + C::SX + 4 * (8 * nt + 2 * t));
 #pragma unroll
             for (int r = 0; r < C::RW; ++r)
 #pragma unroll
@@ -320,6 +311,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
     }
     cp_async_wait<0>();
     __syncthreads();                           // the stages are done with
+    const int rank = min(max(rank_there, 0), P.rank);
     float* sums = reinterpret_cast<float*>(area);
 #pragma unroll
     for (int r = 0; r < C::RW; ++r)
@@ -327,10 +319,10 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                sums[(wk * C::TOK + 32 * wn + 8 * nt + 2 * t + (e & 1)) * C::LDP + 16 * (C::RW * wr + r) + g + 8 * (e >> 1)] = h[r][nt][e];
+                sums[(wk * AD_TOK + 8 * nt + 2 * t + (e & 1)) * C::LDP + 16 * (C::RW * wr + r) + g + 8 * (e >> 1)] = h[r][nt][e];
     __syncthreads();
     // ---- four ranks of a token at a time: this CTA's sums, to a slot in every other CTA of the cluster, and all CTAs' in their order
-    constexpr int QUADS = (C::R * C::TOK / 4 + AD_THREADS - 1) / AD_THREADS;
+    constexpr int QUADS = (C::R * AD_TOK / 4 + AD_THREADS - 1) / AD_THREADS;
     float4 own[QUADS];
     bool ok = true;
     if (parts > 1) cluster_wait();
@@ -338,10 +330,10 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
     for (int m = 0; m < QUADS; ++m) {
         const int i = tid + m * AD_THREADS, n = 4 * i / C::R, j = 4 * i % C::R;
         own[m] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (n < C::TOK) {
+        if (n < AD_TOK) {
 #pragma unroll
             for (int k = 0; k < C::WK; ++k) {
-                const float4 u = *reinterpret_cast<const float4*>(sums + (k * C::TOK + n) * C::LDP + j);
+                const float4 u = *reinterpret_cast<const float4*>(sums + (k * AD_TOK + n) * C::LDP + j);
                 own[m].x += u.x; own[m].y += u.y; own[m].z += u.z; own[m].w += u.w;
             }
             for (int k = 0; k < parts; ++k)
@@ -358,7 +350,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
 #pragma unroll
         for (int m = 0; m < QUADS; ++m) {
             const int i = tid + m * AD_THREADS, n = 4 * i / C::R, j = 4 * i % C::R;
-            if (n >= C::TOK) break;
+            if (n >= AD_TOK) break;
             float v[4] = {};
 #pragma unroll 4
             for (int k = 0; k < parts; ++k) {
@@ -388,8 +380,8 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
         // ---- Y, 128 rows at a time on tcgen05: B as tf32 into its tile, both parts of H times it into tensor memory, from there a thread to a row
         ptx::tc_fence_after();
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 20), wtile = area_s;
-        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = idesc_tf32(128, C::TOK);
-        constexpr int CH = C::R / 8, LOADS = 128 * CH / AD_THREADS, HALF = C::TOK / 2;
+        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = idesc_tf32(128, AD_TOK);
+        constexpr int CH = C::R / 8, LOADS = 128 * CH / AD_THREADS, HALF = AD_TOK / 2;
         uint4 wr16[LOADS];
         auto load_w = [&](int c) {
 #pragma unroll
@@ -470,7 +462,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
             if (issued) ptx::mbar_wait(bar + 8, (issued - 1) & 1, abort_flag);
         }
         __syncthreads();
-        if (warp == 0) ptx::tmem_dealloc(tmem, C::TOK);
+        if (warp == 0) ptx::tmem_dealloc(tmem, AD_TOK);
     } else {
         if (!ok) {
             if (tid == 0) {
@@ -481,10 +473,10 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
             __syncthreads();
             return;
         }
-        if (rank == 0 || nn >= live) return;
+        if (rank == 0) return;
         // ---- Y, a warp for 32 rows and 32 tokens
 #pragma unroll 1
-        for (int c = c0; c < end; c += AD_WARPS / C::WN) {
+        for (int c = c0; c < end; c += AD_WARPS) {
             const int row = 32 * c + 4 * g;
             const bool mine = row < P.rows;
             if (!EARLY && c == c0) load_b(braw, c, 0);         // of the ranks that follow, and of the next rows, they are loaded one step ahead
@@ -503,20 +495,29 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
                         if (j + e >= rank) w[i][e] = 0u;       // nor what B has there
                 }
                 const bool last = 16 * rt + 16 >= rank;
-                if (!last || c + AD_WARPS / C::WN < end) load_b(braw, last ? c + AD_WARPS / C::WN : c, last ? 0 : rt + 1);
+                if (!last || c + AD_WARPS < end) load_b(braw, last ? c + AD_WARPS : c, last ? 0 : rt + 1);
+                // two eights of tokens at a time, and no product right behind another one into the same accumulator
 #pragma unroll
-                for (int nt = 0; nt < 4; ++nt) {
-                    const uint8_t* src = hs + ((nn + 8 * nt + g) * C::LDH + j) * 8;
-                    const float4 u = *reinterpret_cast<const float4*>(src), v = *reinterpret_cast<const float4*>(src + 16);
-                    const uint32_t hi[4] = {__float_as_uint(u.x), __float_as_uint(u.z), __float_as_uint(v.x), __float_as_uint(v.z)};
-                    const uint32_t lo[4] = {__float_as_uint(u.y), __float_as_uint(u.w), __float_as_uint(v.y), __float_as_uint(v.w)};
+                for (int n2 = 0; n2 < 4; n2 += 2) {
+                    uint32_t hi[2][4], lo[2][4];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const uint8_t* src = hs + ((8 * (n2 + nt) + g) * C::LDH + j) * 8;
+                        const uint4 u = *reinterpret_cast<const uint4*>(src), v = *reinterpret_cast<const uint4*>(src + 16);
+                        hi[nt][0] = u.x; lo[nt][0] = u.y; hi[nt][1] = u.z; lo[nt][1] = u.w;
+                        hi[nt][2] = v.x; lo[nt][2] = v.y; hi[nt][3] = v.z; lo[nt][3] = v.w;
+                    }
 #pragma unroll
-                        for (int k = 0; k < 4; k += 2) {
-                            mma_tf32(acc[i][nt], w[2 * i][k], w[2 * i + 1][k], w[2 * i][k + 1], w[2 * i + 1][k + 1], lo[k], lo[k + 1]);
-                            mma_tf32(acc[i][nt], w[2 * i][k], w[2 * i + 1][k], w[2 * i][k + 1], w[2 * i + 1][k + 1], hi[k], hi[k + 1]);
-                        }
+                    for (int k = 0; k < 4; k += 2)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const uint32_t(&x)[4] = e ? hi[nt] : lo[nt];
+                                    mma_tf32(acc[i][n2 + nt], w[2 * i][k], w[2 * i + 1][k], w[2 * i][k + 1], w[2 * i + 1][k + 1], x[k], x[k + 1]);
+                                }
                 }
             }
             if (!mine) continue;
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
             for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int n = nn + 8 * nt + 2 * t + e;
+                    const int n = 8 * nt + 2 * t + e;
                     if (n >= live) continue;
                     add_to4(yrow + n * p.ldy, acc[0][nt][e], acc[0][nt][2 + e], acc[1][nt][e], acc[1][nt][2 + e]);
                 }
@@ -536,43 +537,34 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : RT * NT <= 32 ? 2 : 
 }  // namespace llattn
 
 namespace {
-// Tokens of a tile and CTAs of a cluster, by the sizes alone (the segments are on the device).
-struct AdapterForm { int tok, parts; long long tiles; };
-AdapterForm adapter_form(long long ntokens, long long nseg, int npools, int rt, int sms) {
-    AdapterForm f{};
-    using namespace llattn;
-    f.tok = rt >= 4 && ntokens >= 128 * nseg && ntokens * npools >= 1024 ? 64 : 32;
-    // no more tiles than this, however the segments cut the tokens: each has at most one that is not full
-    f.tiles = std::min(ntokens, (ntokens + (f.tok - 1) * nseg) / f.tok);
-    const long long full = std::max(std::min(nseg, ntokens), (ntokens + f.tok - 1) / f.tok);
-    const int most = rt < 8 ? (f.tok == 32 ? 8 : AdapterTile<4, 8>::MOST) : f.tok == 32 ? AdapterTile<8, 4>::MOST : AdapterTile<8, 8>::MOST;
-    f.parts = 1;
-    while (f.parts < most && 2 * f.parts * full * npools <= 2 * sms) f.parts *= 2;
-    return f;
+// CTAs of a cluster, by the sizes alone (the segments are on the device): as many as fit on the chip at once, two an SM where their shared memory lets
+// them. In a graph, with 1 / 2 / 4 / 8 of them: rank 16, 1 token 14.2 / 8.8 / 6.2 / 5.0 us, 64 segments of 32 tokens 21.6 / 14.1 / 13.4 / 18.2, 4096 tokens
+// 24.4 / 21.4 / 27.7 / -; rank 64, 8 segments of 128 tokens 35.5 / 20.7 / 14.2 / 31, 4096 tokens 35.8 / 31.1 / 37.0 / -.
+template <int RT> int adapter_parts(long long ntokens, long long nseg, int npools, int sms) {
+    const long long tiles = std::max(std::min(nseg, ntokens), (ntokens + llattn::AD_TOK - 1) / llattn::AD_TOK) * npools;
+    int parts = 8;
+    while (parts > 1 && parts * tiles > (llattn::AdapterTile<RT>::bytes(parts) <= 113 * 1024 ? 2 : 1) * sms) parts /= 2;
+    return parts;
 }
 
-template <typename T, int RT, int NT>
-int launch_adapters_tile(llattn::AdapterParams& p, int npools, const AdapterForm& f, cudaStream_t stream) {
+template <typename T, int RT>
+int launch_adapters(llattn::AdapterParams& p, int npools, int sms, cudaStream_t stream) {
     using namespace llattn;
     static std::once_flag once[64];
-    auto* kernel = adapters_kernel<T, RT, NT>;
-    constexpr int most = AdapterTile<RT, NT>::bytes(AdapterTile<RT, NT>::MOST);
+    auto* kernel = adapters_kernel<T, RT>;
+    constexpr int most = AdapterTile<RT>::bytes(8);
+    static_assert(most <= 227 * 1024, "shared memory of the largest cluster");
     int dev = 0;
     CU(cudaGetDevice(&dev));
     if (most > 48 * 1024) {
         if (dev < 0 || dev >= 64) CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         else std::call_once(once[dev], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most); });
     }
-    p.parts = f.parts;
-    CU(launch_dependent_cluster(kernel, dim3(unsigned(f.tiles * f.parts), npools), AD_THREADS, AdapterTile<RT, NT>::bytes(f.parts), f.parts, stream, p));
+    p.parts = adapter_parts<RT>(p.ntokens, p.nseg, npools, sms);
+    // no more tiles than this, however the segments cut the tokens: each has at most one that is not full
+    const long long tiles = std::min<long long>(p.ntokens, (p.ntokens + (AD_TOK - 1ll) * p.nseg) / AD_TOK);
+    CU(launch_dependent_cluster(kernel, dim3(unsigned(tiles * p.parts), npools), AD_THREADS, AdapterTile<RT>::bytes(p.parts), p.parts, stream, p));
     return LLATTN_OK;
-}
-template <typename T, int RT>
-int launch_adapters(llattn::AdapterParams& p, int npools, int sms, cudaStream_t stream) {
-    const AdapterForm f = adapter_form(p.ntokens, p.nseg, npools, RT, sms);
-    if constexpr (RT >= 4)
-        if (f.tok == 64) return launch_adapters_tile<T, RT, 8>(p, npools, f, stream);
-    return launch_adapters_tile<T, RT, 4>(p, npools, f, stream);
 }
 template <typename T>
 int launch_adapters_rank(llattn::AdapterParams& p, int npools, int rank, int sms, cudaStream_t stream) {
