@@ -149,29 +149,34 @@ def _ptr(t) -> Optional[int]:
     return t.data_ptr()
 
 
-def _types():
-    import torch
-    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_torch_of = None
 
 
-_TYPES = None
+def _torch():
+    """(torch, LLATTN_F32 / F16 / BF16 by dtype, the current device's index)"""
+    global _torch_of
+    if _torch_of is None:
+        import torch
+        types, device = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}, getattr(torch._C, "_cuda_getDevice", None)
+        if device is None or not torch.cuda.is_initialized():
+            return torch, types, torch.cuda.current_device()
+        _torch_of = torch, types, device
+    torch, types, device = _torch_of
+    return torch, types, device()
 
 
-def _type_of(t) -> int:
-    """LLATTN_F32, F16 or BF16 of a tensor (-1: none of them)."""
-    global _TYPES
-    if _TYPES is None:
-        _TYPES = _types()
-    return _TYPES.get(t.dtype, -1)
+def _flat(t, dtype, n: int, dev: int, what: str) -> int:
+    """Data pointer of a contiguous tensor of n values on device `dev`, the current one: that is where the launch goes, whatever the pointers."""
+    if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: {n} contiguous values of {dtype} on cuda:{dev}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
-def _here(*tensors) -> None:
-    """Every tensor (None: no tensor) is on the current device: the launch goes to that device, whatever the pointers."""
-    import torch
-    dev = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
+def _rows(t, dtype, T: int, K: int, dev: int, what: str):
+    """Data pointer and row distance of a matrix [T][K] whose rows are contiguous (dtype None: any)."""
+    if t.shape != (T, K) or (dtype is not None and t.dtype is not dtype) or t.get_device() != dev or (K > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: [{T}][{K}] with contiguous rows on cuda:{dev}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr(), (t.stride(0) if T > 1 else K)
 
 
 _raw_stream = None
@@ -340,68 +345,59 @@ def rope_axes(sections, interleaved: bool = False) -> bytes:
     return bytes(out)
 
 
-def _check_axes(qkv, pos, axis_of, gq, gk, inv_freq_t, q, k, v):
-    import torch
+def _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v):
+    torch, _, dev = _torch()
     T = qkv.shape[0]
-    if qkv.shape != (T, (NQH + 2 * NKV) * D) or qkv.dtype != torch.float32 or pos.dim() != 2 or pos.shape[1] != T or pos.dtype != torch.int32:
-        raise ValueError("qkv is fp32 [T][3072], pos int32 [axes][T]")
-    if len(axis_of) != 32:
-        raise ValueError("axis_of has one axis for each of the 32 frequencies")
-    if any(t.numel() != n or t.dtype != torch.float32 for t, n in ((gq, D), (gk, D), (inv_freq_t, 32))):
-        raise ValueError("gq and gk are fp32 [128], inv_freq fp32 [32]")
-    if any(t.numel() != T * n * D or t.dtype != torch.float16 for t, n in ((q, NQH), (k, NKV), (v, NKV))):
-        raise ValueError("q is fp16 [T][16][128], k and v fp16 [T][4][128]")
-    return T
+    if pos.dim() != 2 or pos.shape[1] != T or len(axis_of) != 32:
+        raise ValueError("pos is int32 [axes][T], axis_of one axis for each of the 32 frequencies")
+    f32, f16, naxes = torch.float32, torch.float16, pos.shape[0]
+    return T, (_flat(qkv, f32, T * (NQH + 2 * NKV) * D, dev, "qkv"), _flat(pos, torch.int32, naxes * T, dev, "pos"), naxes, bytes(axis_of),
+               _flat(gq, f32, D, dev, "gq"), _flat(gk, f32, D, dev, "gk"), eps, _flat(inv_freq_t, f32, 32, dev, "inv_freq"),
+               _flat(q, f16, T * NQH * D, dev, "q"), _flat(k, f16, T * NKV * D, dev, "k"), _flat(v, f16, T * NKV * D, dev, "v"))
 
 
 def qk_norm_rope_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream=None) -> None:
     """qk_norm_rope with several position axes: pos int32 [axes][T], axis_of the axis of each of the 32 frequencies (host; see rope_axes)."""
-    T = _check_axes(qkv, pos, axis_of, gq, gk, inv_freq_t, q, k, v)
-    _here(qkv, pos, gq, gk, inv_freq_t, q, k, v)
-    _check(lib().llattn_qk_norm_rope_axes(_ptr(qkv), _ptr(pos), pos.shape[0], bytes(axis_of), _ptr(gq), _ptr(gk), eps, _ptr(inv_freq_t), _ptr(q),
-                                          _ptr(k), _ptr(v), T, _stream(stream)))
+    T, args = _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v)
+    _check(lib().llattn_qk_norm_rope_axes(*args, T, _stream(stream)))
 
 
 def qkv_prepare_commit_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, cache, max_blocks: int = 0, blk: int = 0, pages=None,
                             stream=None) -> None:
     """qkv_prepare_commit with several position axes, see qk_norm_rope_axes."""
-    T = _check_axes(qkv, pos, axis_of, gq, gk, inv_freq_t, q, k, v)
+    T, args = _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v)
+    torch, _, dev = _torch()
+    nb = T // BLK
     if T % BLK:
         raise ValueError("a prefill pass commits whole 32-token blocks")
-    if pages is not None and pages.numel() != T // BLK * NKV:
-        raise ValueError("pages must hold nb * 4 indices")
-    _here(qkv, pos, gq, gk, inv_freq_t, q, k, v, cache, pages)
-    _check(lib().llattn_qkv_prepare_commit_axes(_ptr(qkv), _ptr(pos), pos.shape[0], bytes(axis_of), _ptr(gq), _ptr(gk), eps, _ptr(inv_freq_t),
-                                                _ptr(q), _ptr(k), _ptr(v), T // BLK, _ptr(cache), _ptr(pages), max_blocks, blk, _stream(stream)))
+    if pages is None and cache.numel() < NKV * max_blocks * KV_BLOCK_BYTES:
+        raise ValueError("the cache holds fewer than max_blocks blocks")
+    _check(lib().llattn_qkv_prepare_commit_axes(*args, nb, _flat(cache, torch.uint8, cache.numel(), dev, "cache"),
+                                                None if pages is None else _flat(pages, torch.int32, nb * NKV, dev, "pages"), max_blocks, blk, _stream(stream)))
 
 
 # ------------------------------------------------------------------ norm, adapters
-
-def _rows(t, K: int, what: str):
-    """Data pointer and row distance of a matrix whose rows are contiguous."""
-    if t.dim() != 2 or t.shape[1] != K or (K > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: [T][{K}] with contiguous rows")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else K)
-
 
 def add_norm_q8(x, gain, eps, q=None, s=None, qsum=None, delta=None, y=None, stream=None) -> None:
     """Residual addition, RMS norm and int8 activations in one pass (llattn_add_norm_q8). x fp32 [T][K] takes delta (fp32, fp16 or bf16 [T][K];
     None: nothing is added and x is only read); q int8 [T][K] in fragment order, s fp32 and qsum int32 [T][K/128] are what dense_w4a8 and
     adapters_w4a8 read; y fp16 or bf16 [T][K] the normalised values. The rows of x and delta may be further apart than K."""
-    import torch
+    torch, types, dev = _torch()
     T, K = x.shape
-    xp, ldx = _rows(x, K, "x")
-    dp, ldd = (None, 0) if delta is None else _rows(delta, K, "delta")
-    if x.dtype != torch.float32 or gain.dtype != torch.float32 or gain.numel() != K or (delta is not None and delta.shape[0] != T):
-        raise ValueError("x and gain are fp32, [T][K] and [K], delta [T][K]")
-    if q is not None and (q.shape != x.shape or q.dtype != torch.int8 or s is None or qsum is None or s.shape != (T, K // 128) or s.dtype != torch.float32 or
-                          qsum.shape != s.shape or qsum.dtype != torch.int32):
-        raise ValueError("q is int8 [T][K], s fp32 and qsum int32 [T][K / 128]")
-    if y is not None and y.shape != x.shape:
-        raise ValueError("y is [T][K]")
-    _here(x, gain, q, s, qsum, delta, y)
-    _check(lib().llattn_add_norm_q8(xp, ldx, dp, 0 if delta is None else _type_of(delta), ldd, _ptr(gain), eps, _ptr(q), _ptr(s), _ptr(qsum),
-                                    _ptr(y), 0 if y is None else _type_of(y), T, K, _stream(stream)))
+    xp, ldx = _rows(x, torch.float32, T, K, dev, "x")
+    dp, ldd, dtype, qp, sp, sump, yp, ytype = None, 0, 0, None, None, None, None, 0
+    if delta is not None:
+        dp, ldd = _rows(delta, None, T, K, dev, "delta")
+        dtype = types.get(delta.dtype, -1)
+    if q is not None:
+        if s is None or qsum is None:
+            raise ValueError("q, s and qsum go together")
+        qp, sp, sump = _flat(q, torch.int8, T * K, dev, "q"), _flat(s, torch.float32, T * (K // 128), dev, "s"), _flat(qsum, torch.int32, T * (K // 128), dev, "qsum")
+    elif s is not None or qsum is not None:
+        raise ValueError("q, s and qsum go together")
+    if y is not None:
+        yp, ytype = _flat(y, y.dtype, T * K, dev, "y"), types.get(y.dtype, -1)
+    _check(lib().llattn_add_norm_q8(xp, ldx, dp, dtype, ldd, _flat(gain, torch.float32, K, dev, "gain"), eps, qp, sp, sump, yp, ytype, T, K, _stream(stream)))
 
 
 @dataclass
@@ -423,7 +419,7 @@ class AdapterPool:
         if (self.scale is not None and (self.scale.numel() != n or self.scale.dtype != torch.float32)) or \
            (self.ranks is not None and (self.ranks.numel() != n or self.ranks.dtype != torch.int32)):
             raise ValueError("scale is fp32 [n], ranks int32 [n]")
-        return _AdapterPool(_ptr(A), _ptr(B), _ptr(self.scale), _ptr(self.ranks), n, A.shape[1], B.shape[1], self.row0, _type_of(A))
+        return _AdapterPool(_ptr(A), _ptr(B), _ptr(self.scale), _ptr(self.ranks), n, A.shape[1], B.shape[1], self.row0, _torch()[1].get(A.dtype, -1))
 
 
 class AdapterPools:
@@ -438,6 +434,7 @@ class AdapterPools:
         if any(t is not None and t.get_device() != self.device for p in self.pools for t in (p.A, p.B, p.scale, p.ranks)):
             raise ValueError("the pools are on one device")
         self._c = (_AdapterPool * len(self.pools))(*[p._c() for p in self.pools])
+        self._rows = max(p.row0 + p.B.shape[1] for p in self.pools)
 
 
 def adapter_pools(pools: Sequence[AdapterPool]) -> AdapterPools:
@@ -448,19 +445,14 @@ def adapters_w4a8(pools: AdapterPools, q, s, Y, seg_first, seg_adapter, stream=N
     """Adds the adapters of many requests to a projection's output Y (fp32 [ntokens][>= row0 + rows], rows contiguous), from the activations
     (q int8 [ntokens][K] in fragment order, s fp32 [ntokens][K/128]) that dense_w4a8 reads (llattn_adapters_w4a8). Segment i is the tokens
     seg_first[i] .. seg_first[i + 1] - 1 and has adapter seg_adapter[i] (-1: none); both are int32 device tensors."""
-    import torch
-    T, K = q.shape
-    yp, ldy = _rows(Y, Y.shape[-1], "Y")
-    nseg = seg_adapter.numel()
-    if K != pools.K or q.dtype != torch.int8 or s.shape != (T, K // 128) or s.dtype != torch.float32 or Y.shape[0] != T or Y.dtype != torch.float32:
-        raise ValueError(f"q is int8 [T][{pools.K}], s fp32 [T][{pools.K // 128}], Y fp32 [T][..]")
-    if seg_first.numel() != nseg + 1 or seg_first.dtype != torch.int32 or seg_adapter.dtype != torch.int32:
-        raise ValueError("seg_first is int32 [segments + 1], seg_adapter int32 [segments]")
-    if any(p.row0 + p.B.shape[1] > Y.shape[1] for p in pools.pools):
-        raise ValueError("a pool's rows reach beyond Y's")
-    _here(pools.pools[0].A, q, s, Y, seg_first, seg_adapter)
-    _check(lib().llattn_adapters_w4a8(pools._c, len(pools.pools), _ptr(q), _ptr(s), yp, ldy, T, K, _ptr(seg_first), _ptr(seg_adapter), nseg,
-                                      _stream(stream)))
+    torch, _, dev = _torch()
+    T, width = Y.shape
+    K, nseg, f32, i32 = pools.K, seg_adapter.numel(), torch.float32, torch.int32
+    if pools._rows > width or pools.device != dev:
+        raise ValueError(f"the pools' rows reach to {pools._rows} of {width}, on cuda:{pools.device}; the current device is cuda:{dev}")
+    yp, ldy = _rows(Y, f32, T, width, dev, "Y")
+    _check(lib().llattn_adapters_w4a8(pools._c, len(pools._c), _flat(q, torch.int8, T * K, dev, "q"), _flat(s, f32, T * (K // 128), dev, "s"), yp, ldy, T, K,
+                                      _flat(seg_first, i32, nseg + 1, dev, "seg_first"), _flat(seg_adapter, i32, nseg, dev, "seg_adapter"), nseg, _stream(stream)))
 
 
 # ------------------------------------------------------------------ the reference operator pair

@@ -11,6 +11,7 @@
 // A lane holds four neighbouring values of a group (a run of four stays together in fragment order), a warp the group: maximum and code sum
 // are one redux instruction each. W warps share a row, group by group in turn; the row's sum of squares is folded lane-wise over a warp's
 // groups, by a butterfly over the lanes and over the warps in order, all in fp32.
+// Bound by memory from a few thousand rows on (8191 x 2048 with an fp32 addend 37.9 us = 5.8 TB/s), below by the launch and one round trip.
 #pragma once
 
 namespace llattn {
@@ -66,7 +67,8 @@ __device__ __forceinline__ uint2 norm_pack16(const float4& v, int type) {
     return w;
 }
 
-template <int DTYPE, int W, int ROWS>
+// W warps share a row, ROWS rows are in a CTA. A warp has the loads of G of its groups in flight.
+template <int DTYPE, int W, int ROWS, int G>
 __global__ void __launch_bounds__(32 * W * ROWS) add_norm_q8_kernel(const NormQ8Params p) {
     __shared__ float steps[ROWS][NQ_MAX_GROUPS];
     __shared__ float parts[ROWS][W];
@@ -74,37 +76,49 @@ __global__ void __launch_bounds__(32 * W * ROWS) add_norm_q8_kernel(const NormQ8
     const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) % W, rr = (threadIdx.x >> 5) / W;
     const int row = blockIdx.x * ROWS + rr, groups = p.K / NQ_GROUP;
     const bool live = row < p.T;
-    float* x = p.x + (long long)row * p.ldx;
-    const size_t drow = DTYPE == NQ_NONE ? 0 : size_t(row) * p.ldd;
+    float* x = p.x + (long long)row * p.ldx + 4 * lane;
+    const size_t drow = DTYPE == NQ_NONE ? 0 : size_t(row) * p.ldd + 4 * lane;
+    const float* gain = p.gain + 4 * lane;
+    const size_t out = size_t(row) * p.K;
     float ss = 0.f;
+    float4 v[G];
     if (live) {
-#pragma unroll 4
-        for (int g = w; g < groups; g += W) {
-            const int at = g * NQ_GROUP + 4 * lane;
-            float4 v = *reinterpret_cast<const float4*>(x + at);
-            const float4 gn = __ldg(reinterpret_cast<const float4*>(p.gain + at));
-            if constexpr (DTYPE != NQ_NONE) {
-                const float4 d = norm_load<DTYPE>(p.d, drow + at);
-                v.x += d.x; v.y += d.y; v.z += d.z; v.w += d.w;
-                *reinterpret_cast<float4*>(x + at) = v;
-            }
-            ss += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
-            if (p.q) {
-                const float t0 = __fmul_rn(v.x, gn.x), t1 = __fmul_rn(v.y, gn.y), t2 = __fmul_rn(v.z, gn.z), t3 = __fmul_rn(v.w, gn.w);
-                // of non-negative floats the bits order as the values do, and NaN is above infinity
-                const uint32_t most = max(max(__float_as_uint(fabsf(t0)), __float_as_uint(fabsf(t1))), max(__float_as_uint(fabsf(t2)), __float_as_uint(fabsf(t3))));
-                const float a = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
-                const bool finite = a < INFINITY;
-                const float e = finite ? fmaxf(__fdiv_rn(a, 127.f), 1e-30f) : __uint_as_float(0x7fc00000u);      // else the group's scale is NaN, its codes 0
-                const float inv = __frcp_rn(e);
-                uint32_t word = 0;
-                if (finite) word = __byte_perm(__byte_perm(norm_code(t0, e, inv), norm_code(t1, e, inv), 0x0040),
-                                               __byte_perm(norm_code(t2, e, inv), norm_code(t3, e, inv), 0x0040), 0x5410);
-                const int total = __reduce_add_sync(0xffffffffu, __dp4a(int(word), 0x01010101, 0));
-                *reinterpret_cast<uint32_t*>(p.q + size_t(row) * p.K + frag_pos(at)) = word;
-                if (lane == 0) {
-                    steps[rr][g] = e;
-                    p.sum[size_t(row) * groups + g] = total;
+#pragma unroll 1
+        for (int g0 = w; g0 < groups; g0 += W * G) {
+            float4 d[G];
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+                if (g0 + i * W < groups) {
+                    v[i] = *reinterpret_cast<const float4*>(x + (g0 + i * W) * NQ_GROUP);
+                    if constexpr (DTYPE != NQ_NONE) d[i] = norm_load<DTYPE>(p.d, drow + (g0 + i * W) * NQ_GROUP);
+                }
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                const int g = g0 + i * W;
+                if (g >= groups) break;
+                if constexpr (DTYPE != NQ_NONE) {
+                    v[i].x += d[i].x; v[i].y += d[i].y; v[i].z += d[i].z; v[i].w += d[i].w;
+                    *reinterpret_cast<float4*>(x + g * NQ_GROUP) = v[i];
+                }
+                ss += v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w;
+                const float4 gn = __ldg(reinterpret_cast<const float4*>(gain + g * NQ_GROUP));
+                v[i] = make_float4(__fmul_rn(v[i].x, gn.x), __fmul_rn(v[i].y, gn.y), __fmul_rn(v[i].z, gn.z), __fmul_rn(v[i].w, gn.w));
+                if (p.q) {
+                    // of non-negative floats the bits order as the values do, and NaN is above infinity
+                    const uint32_t most = max(max(__float_as_uint(fabsf(v[i].x)), __float_as_uint(fabsf(v[i].y))), max(__float_as_uint(fabsf(v[i].z)), __float_as_uint(fabsf(v[i].w))));
+                    const float a = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
+                    const bool finite = a < INFINITY;
+                    const float e = finite ? fmaxf(__fdiv_rn(a, 127.f), 1e-30f) : __uint_as_float(0x7fc00000u);      // else the group's scale is NaN, its codes 0
+                    const float inv = __frcp_rn(e);
+                    uint32_t word = 0;
+                    if (finite) word = __byte_perm(__byte_perm(norm_code(v[i].x, e, inv), norm_code(v[i].y, e, inv), 0x0040),
+                                                   __byte_perm(norm_code(v[i].z, e, inv), norm_code(v[i].w, e, inv), 0x0040), 0x5410);
+                    const int total = __reduce_add_sync(0xffffffffu, __dp4a(int(word), 0x01010101, 0));
+                    *reinterpret_cast<uint32_t*>(p.q + out + frag_pos(g * NQ_GROUP + 4 * lane)) = word;
+                    if (lane == 0) {
+                        steps[rr][g] = e;
+                        p.sum[size_t(row) * groups + g] = total;
+                    }
                 }
             }
         }
@@ -120,23 +134,38 @@ __global__ void __launch_bounds__(32 * W * ROWS) add_norm_q8_kernel(const NormQ8
     const float r = rsqrtf(ss / float(p.K) + p.eps);
     if (p.q)
         for (int g = 32 * w + lane; g < groups; g += 32 * W) p.s[size_t(row) * groups + g] = __fmul_rn(steps[rr][g], r);
-    if (p.y)
-        for (int g = w; g < groups; g += W) {          // the values that this thread has read, or written, above
-            const int at = g * NQ_GROUP + 4 * lane;
-            const float4 v = *reinterpret_cast<const float4*>(x + at);
-            const float4 gn = __ldg(reinterpret_cast<const float4*>(p.gain + at));
-            const float4 t = make_float4(__fmul_rn(__fmul_rn(v.x, gn.x), r), __fmul_rn(__fmul_rn(v.y, gn.y), r), __fmul_rn(__fmul_rn(v.z, gn.z), r), __fmul_rn(__fmul_rn(v.w, gn.w), r));
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + size_t(row) * p.K + at) = norm_pack16(t, p.y_type);
-        }
+    if (p.y) {
+        uint16_t* y = static_cast<uint16_t*>(p.y) + out + 4 * lane;
+        auto store = [&](int g, const float4& t) {
+            *reinterpret_cast<uint2*>(y + g * NQ_GROUP) = norm_pack16(make_float4(__fmul_rn(t.x, r), __fmul_rn(t.y, r), __fmul_rn(t.z, r), __fmul_rn(t.w, r)), p.y_type);
+        };
+        if (groups <= W * G) {                 // t is still in the registers
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+                if (w + i * W < groups) store(w + i * W, v[i]);
+        } else
+            for (int g = w; g < groups; g += W) {      // what this thread has read, or written, above
+                const float4 u = *reinterpret_cast<const float4*>(x + g * NQ_GROUP);
+                const float4 gn = __ldg(reinterpret_cast<const float4*>(gain + g * NQ_GROUP));
+                store(g, make_float4(__fmul_rn(u.x, gn.x), __fmul_rn(u.y, gn.y), __fmul_rn(u.z, gn.z), __fmul_rn(u.w, gn.w)));
+            }
+    }
 }
 
 }  // namespace llattn
 
 namespace {
+// How a row is shared. Few rows, or long ones: many warps a row, so that the chip is filled and the chain of a warp short. Many rows: few warps a row, each
+// with several groups of loads in flight. In a graph, rows x K, with 16 / 8 / 4 / 2 warps a row: 1 x 2048 2.0 / 2.4 / 3.1 / 6.0 us, 256 x 2048 2.8 / 2.9 /
+// 3.6 / 6.9, 512 x 2048 4.7 / 3.9 / 5.4 / 7.9, 515 x 5120 11.2 / 10.1 / 13.4 / 22.9, 1024 x 2048 7.8 / 8.1 / 7.3 / 10.2, 2048 x 2048 13.2 / 13.1 / 12.5 / 13.3,
+// 8191 x 2048 46.7 / 41.3 / 39.9 / 37.9, 2000 x 512 9.0 / 7.1 / 4.4 / 3.9, 2048 x 8192 36.2 / 39.2 / 42.4 / 45.1.
 template <int DTYPE>
 cudaError_t launch_norm_q8(const llattn::NormQ8Params& p, int sms, cudaStream_t stream) {
-    if (p.T <= sms) return launch_dependent(llattn::add_norm_q8_kernel<DTYPE, 16, 1>, dim3(p.T), 512, stream, p);
-    return launch_dependent(llattn::add_norm_q8_kernel<DTYPE, 4, 2>, dim3((p.T + 1) / 2), 256, stream, p);
+    const int groups = p.K / llattn::NQ_GROUP;
+    if (p.T <= 2 * sms || (groups >= 64 && p.T > 4 * sms)) return launch_dependent(llattn::add_norm_q8_kernel<DTYPE, 16, 1, 1>, dim3(p.T), 512, stream, p);
+    if (p.T <= 4 * sms || groups >= 32) return launch_dependent(llattn::add_norm_q8_kernel<DTYPE, 8, 1, 2>, dim3(p.T), 256, stream, p);
+    if (p.T <= 32 * sms && groups >= 8) return launch_dependent(llattn::add_norm_q8_kernel<DTYPE, 4, 2, 1>, dim3((p.T + 1) / 2), 256, stream, p);
+    return launch_dependent(llattn::add_norm_q8_kernel<DTYPE, 2, 4, 2>, dim3((p.T + 3) / 4), 256, stream, p);
 }
 
 // Whether two ranges of bytes have one in common.
