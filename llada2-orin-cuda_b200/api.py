@@ -174,9 +174,13 @@ def _flat(t, dtype, n: int, dev: int, what: str) -> int:
 
 def _rows(t, dtype, T: int, K: int, dev: int, what: str):
     """Data pointer and row distance of a matrix [T][K] whose rows are contiguous (dtype None: any)."""
-    if t.shape != (T, K) or (dtype is not None and t.dtype is not dtype) or t.get_device() != dev or (K > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: [{T}][{K}] with contiguous rows on cuda:{dev}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
-    return t.data_ptr(), (t.stride(0) if T > 1 else K)
+    if t.numel() == T * K and t.get_device() == dev and (dtype is None or t.dtype is dtype) and t.shape[-1] == K:
+        if t.is_contiguous():
+            return t.data_ptr(), K
+        strides = t.stride()
+        if len(strides) == 2 and (strides[1] == 1 or K == 1):
+            return t.data_ptr(), (strides[0] if T > 1 else K)
+    raise ValueError(f"{what}: [{T}][{K}] with contiguous rows on cuda:{dev}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
 
 
 _raw_stream = None

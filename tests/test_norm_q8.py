@@ -88,7 +88,8 @@ def _check(orc, x, d, gain, eps, got, y_type=None):
         assert (np.abs(gy - y) <= (half + tol * 1.01) * np.abs(y) + (2.0 ** -25 if y_type == torch.float16 else 0)).all()
 
 
-SIZES = [(1, 128), (1, 2048), (3, 384), (32, 2048), (5, 32768), (147, 640), (148, 2048), (149, 2048), (150, 128), (301, 2176), (515, 5120), (200, 32768), (1000, 256)]
+SIZES = [(1, 128), (1, 2048), (3, 384), (32, 2048), (5, 32768), (147, 640), (148, 2048), (149, 2048), (150, 128), (301, 2176), (515, 5120), (200, 32768), (1000, 256), (296, 384), (297, 384), (592, 1024), (593, 1024), (593, 896),
+         (700, 4096), (592, 8192), (593, 8192), (4736, 1024), (4737, 1024)]
 
 
 @pytest.mark.gpu
