@@ -106,9 +106,9 @@ template <int RT> struct AdapterTile {
     // the cluster.
     static constexpr bool WIDE = RT >= 4;
     static constexpr int LDP = R + 4, LDH = R + 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
-    static constexpr int WBLOCK = 128 * 128, HBLOCK = TOK * 128, HPART = R / 32 * HBLOCK;       // 32 ranks of 128 rows, of the tokens; all of them
+    static constexpr int WBLOCK = 128 * 128, HBLOCK = 2 * TOK * 128;       // 32 ranks of 128 rows, of the tokens' values and of their remainders
     static constexpr int H_AT = !WIDE ? SUMS : (SUMS > R / 32 * WBLOCK ? (SUMS + 1023) / 1024 * 1024 : R / 32 * WBLOCK);
-    static constexpr int AREA = H_AT + (WIDE ? 2 * HPART : TOK * LDH * 8);
+    static constexpr int AREA = H_AT + (WIDE ? R / 32 * HBLOCK : TOK * LDH * 8);
     static constexpr int HEAD = WIDE ? 1024 : 64;
     static constexpr int bytes(int ctas) { return HEAD + (ctas - 1) * SLOT + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
 };
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
     };
     for (int i = 0; i < C::STAGES - 1; ++i) fetch(i);
     if constexpr (C::WIDE)
-        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), AD_TOK); ptx::tmem_relinquish(); }
+        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), 2 * AD_TOK); ptx::tmem_relinquish(); }
     const int rank_there = P.ranks ? __ldg(P.ranks + a) : P.rank;  // looked at when the sums are there: a wait for it here would hold up what follows
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
     // ---- this CTA's rows of B are wanted when H is done: into L2, and a small rank's first ones into registers
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             if constexpr (C::WIDE) {
                 uint8_t* to = hs + j / 32 * C::HBLOCK + n * 128 + ((j % 32 / 4 ^ (n & 7)) << 4);
                 *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(to + C::HPART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                *reinterpret_cast<uint4*>(to + AD_TOK * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             } else {
                 uint4* to = reinterpret_cast<uint4*>(hs + (n * C::LDH + j) * 8);
                 to[0] = make_uint4(hi[0], lo[0], hi[1], lo[1]);
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         // ---- Y, 128 rows at a time on tcgen05: B as tf32 into its tile, both parts of H times it into tensor memory, from there a thread to a row
         ptx::tc_fence_after();
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 20), wtile = area_s;
-        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = idesc_tf32(128, AD_TOK);
+        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = idesc_tf32(128, 2 * AD_TOK);
         constexpr int CH = C::R / 8, LOADS = 128 * CH / AD_THREADS, HALF = AD_TOK / 2;
         uint4 wr16[LOADS];
         auto load_w = [&](int c) {
@@ -424,24 +424,27 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             if (warp == 0) {
 #pragma unroll 1
                 for (int k = 0; 32 * k < rank; ++k) {
-                    const uint32_t wa = ptx::desc_lo(wtile + k * C::WBLOCK, 16), ha = ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16);
-                    mma_tf32_block_warp(tmem, wa, ha + C::HPART / 16, dhi, idesc, k > 0);
-                    mma_tf32_block_warp(tmem, wa, ha, dhi, idesc, 1);
+                    mma_tf32_block_warp(tmem, ptx::desc_lo(wtile + k * C::WBLOCK, 16), ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16), dhi, idesc, k > 0);
                 }
                 ptx::mma_commit_warp(bar + 8);
             }
             load_w(c + 1);
             ok = ptx::mbar_wait_warp(bar + 8, (c - first) & 1, abort_flag);
             ptx::tc_fence_after();
-            // rows 4 g and + 1 in a, + 2 and + 3 in b; tokens 8 i + 2 t and + 1
-            uint32_t ra[HALF / 2], rb[HALF / 2];
+            // rows 4 g and + 1 in the first, + 2 and + 3 in the second; tokens 8 i + 2 t and + 1; the remainders' part 32 columns on
+            uint32_t ra[HALF / 2], rb[HALF / 2], qa[HALF / 2], qb[HALF / 2];
             const int nw = HALF * (warp >> 2), row = 128 * c + 32 * (warp & 3) + 4 * g;
             const uint32_t from = tmem + (uint32_t(32 * (warp & 3)) << 16) + nw;
             ptx::tmem_ld16x256_cols(from, ra);
             ptx::tmem_ld16x256_cols(from + (16u << 16), rb);
+            ptx::tmem_ld16x256_cols(from + AD_TOK, qa);
+            ptx::tmem_ld16x256_cols(from + (16u << 16) + AD_TOK, qb);
             ptx::tmem_wait_ld_tied(ra);
             ptx::tmem_wait_ld_tied(rb);
+            ptx::tmem_wait_ld_tied(qa);
+            ptx::tmem_wait_ld_tied(qb);
             ptx::tc_fence_before();
+            auto sum = [](uint32_t x, uint32_t y) { return __uint_as_float(x) + __uint_as_float(y); };
             float* yrow = p.Y + (n0 + nw) * p.ldy + P.row0 + row;
             if (ok && row < P.rows)
 #pragma unroll
@@ -450,7 +453,8 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
                     for (int e = 0; e < 2; ++e) {
                         const int n = 8 * i + 2 * t + e;
                         if (nw + n < live)
-                            add_to4(yrow + n * p.ldy, __uint_as_float(ra[4 * i + e]), __uint_as_float(ra[4 * i + 2 + e]), __uint_as_float(rb[4 * i + e]), __uint_as_float(rb[4 * i + 2 + e]));
+                            add_to4(yrow + n * p.ldy, sum(ra[4 * i + e], qa[4 * i + e]), sum(ra[4 * i + 2 + e], qa[4 * i + 2 + e]), sum(rb[4 * i + e], qb[4 * i + e]),
+                                    sum(rb[4 * i + 2 + e], qb[4 * i + 2 + e]));
                     }
         }
         ok = __syncthreads_and(ok);
@@ -462,7 +466,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             if (issued) ptx::mbar_wait(bar + 8, (issued - 1) & 1, abort_flag);
         }
         __syncthreads();
-        if (warp == 0) ptx::tmem_dealloc(tmem, AD_TOK);
+        if (warp == 0) ptx::tmem_dealloc(tmem, 2 * AD_TOK);
     } else {
         if (!ok) {
             if (tid == 0) {
