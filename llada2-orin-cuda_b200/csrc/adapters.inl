@@ -411,8 +411,11 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
                             if (j + e >= rank) f[e] = 0.f;                     // nor what B has there
                     const int g8 = r / 4 % 8;      // row 4 g + i of 32 is the tile's g + 8 i: a thread then gets four neighbouring rows from tensor memory
                     uint8_t* to = area + j / 32 * C::WBLOCK + (r / 32 * 32 + g8 + r % 4 * 8) * 128;
-                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 ^ g8) << 4)) = make_float4(f[0], f[1], f[2], f[3]);
-                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 + 1 ^ g8) << 4)) = make_float4(f[4], f[5], f[6], f[7]);
+                    // of the two halves the odd blocks' lanes store the second first: else they would meet the even ones' in the same banks
+                    const bool odd = j / 32 & 1;
+                    const float4 lo = make_float4(f[0], f[1], f[2], f[3]), hi = make_float4(f[4], f[5], f[6], f[7]);
+                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 + odd ^ g8) << 4)) = odd ? hi : lo;
+                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 + !odd ^ g8) << 4)) = odd ? lo : hi;
                 }
                 ptx::fence_proxy_async_smem();
                 ptx::tc_fence_before();
