@@ -49,6 +49,12 @@ struct AdapterF16 {
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
     static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const half2*>(&w)); }
+    static constexpr int PARTS = 2;            // of H, in fp16: 22 bits of a value, the largest of a token brought to 2^13
+    static __device__ __forceinline__ uint32_t part(float& a, float& b) {      // two values rounded, what is left of them in their place
+        const half2 x = __floats2half2_rn(a, b);
+        a -= __low2float(x); b -= __high2float(x);
+        return *reinterpret_cast<const uint32_t*>(&x);
+    }
 };
 struct AdapterBF16 {
     // a byte v behind 0x43 is the bf16 number 128 + (v & 127), and with its sign bit alone 128 or 256: their difference is v, exact
@@ -65,11 +71,13 @@ struct AdapterBF16 {
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
     static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    static constexpr int PARTS = 3;            // of H, in bf16: 24 bits, and no range to be kept
+    static __device__ __forceinline__ uint32_t part(float& a, float& b) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+        a -= __low2float(x); b -= __high2float(x);
+        return *reinterpret_cast<const uint32_t*>(&x);
+    }
 };
-__device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // 32 ranks: four K-steps of kind::tf32 over 128-byte-swizzle tiles (A: 128 rows of B, B: the tokens' H). One elected lane issues.
 __device__ __forceinline__ void mma_tf32_block_warp(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate_first) {
     asm volatile(
@@ -101,14 +109,14 @@ template <int RT> struct AdapterTile {
     static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WK = AD_WARPS / WR;
     // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
     static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : RT > 1 ? 3 : 5;
-    // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], or the tensor cores' tile of B, and H: for few ranks as pairs
-    // (value, remainder), [TOK][LDH], else as the tensor cores' tiles of both. In front of all a slot [TOK][R] for the sums of each other CTA of
+    // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], or the tensor cores' tile of B, and H: for few ranks as parts
+    // of 16 bits, the first two [TOK] rows LDH bytes apart, the third, and a power of two for each token, else as the tensor cores' tiles of both parts. In front of all a slot [TOK][R] for the sums of each other CTA of
     // the cluster.
     static constexpr bool WIDE = RT >= 4;
-    static constexpr int LDP = R + 4, LDH = R + 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
+    static constexpr int LDP = R + 4, LDH = 4 * R + (RT == 2 ? 64 : 0), LDH3 = LDH / 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
     static constexpr int WBLOCK = 128 * 128, HBLOCK = 2 * TOK * 128;       // 32 ranks of 128 rows, of the tokens' values and of their remainders
     static constexpr int H_AT = !WIDE ? SUMS : (SUMS > R / 32 * WBLOCK ? (SUMS + 1023) / 1024 * 1024 : R / 32 * WBLOCK);
-    static constexpr int AREA = H_AT + (WIDE ? R / 32 * HBLOCK : TOK * LDH * 8);
+    static constexpr int AREA = H_AT + (WIDE ? R / 32 * HBLOCK : TOK * (LDH + LDH3 + 4));
     static constexpr int HEAD = WIDE ? 1024 : 64;
     static constexpr int bytes(int ctas) { return HEAD + (ctas - 1) * SLOT + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
 };
@@ -357,21 +365,35 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
                 const float4 u = k == part ? own[m] : slots[(k - (k > part)) * (C::SLOT / 16) + i];
                 v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
             }
-            uint32_t hi[4], lo[4];
+            float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = j + e < rank ? v[e] * scale : 0.f;             // what A has behind the rank, whatever it is, does not count
-                hi[e] = to_tf32(x);
-                lo[e] = to_tf32(x - __uint_as_float(hi[e]));
-            }
+            for (int e = 0; e < 4; ++e) x[e] = j + e < rank ? v[e] * scale : 0.f;      // what A has behind the rank, whatever it is, does not count
             if constexpr (C::WIDE) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    hi[e] = to_tf32(x[e]);
+                    lo[e] = to_tf32(x[e] - __uint_as_float(hi[e]));
+                }
                 uint8_t* to = hs + j / 32 * C::HBLOCK + n * 128 + ((j % 32 / 4 ^ (n & 7)) << 4);
                 *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                 *reinterpret_cast<uint4*>(to + AD_TOK * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             } else {
-                uint4* to = reinterpret_cast<uint4*>(hs + (n * C::LDH + j) * 8);
-                to[0] = make_uint4(hi[0], lo[0], hi[1], lo[1]);
-                to[1] = make_uint4(hi[2], lo[2], hi[3], lo[3]);
+                if constexpr (T::PARTS == 2) {                     // the token's ranks are with R / 4 neighbouring lanes
+                    float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+                    for (int o = 1; o < C::R / 4; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    const int e = most < INFINITY ? max(int(__float_as_uint(most) >> 23) - 127, -100) : 13;
+                    const float up = __uint_as_float(uint32_t(127 + 13 - e) << 23);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] *= up;
+                    if (j == 0) reinterpret_cast<float*>(hs + AD_TOK * (C::LDH + C::LDH3))[n] = __uint_as_float(uint32_t(127 - 13 + e) << 23);
+                }
+                uint32_t w[T::PARTS][2];
+#pragma unroll
+                for (int k = 0; k < T::PARTS; ++k) { w[k][0] = T::part(x[0], x[1]); w[k][1] = T::part(x[2], x[3]); }
+                *reinterpret_cast<uint4*>(hs + n * C::LDH + 4 * j) = make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
+                if constexpr (T::PARTS == 3) *reinterpret_cast<uint2*>(hs + AD_TOK * C::LDH + n * C::LDH3 + 2 * j) = make_uint2(w[2][0], w[2][1]);
             }
         }
     }
@@ -492,41 +514,37 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             for (int rt = 0; rt < RT; ++rt) {
                 if (16 * rt >= rank) break;
                 const int j = 16 * rt + 4 * t;
-                uint32_t w[4][4];              // [row][j]: exact in tf32
+                // B as it is: a lane's four ranks are its K slots, as in the first product. What B has behind the rank, whatever it is, does not count.
+                const uint32_t m0 = j + 1 < rank ? 0xffffffffu : j < rank ? 0xffffu : 0u, m1 = j + 3 < rank ? 0xffffffffu : j + 2 < rank ? 0xffffu : 0u;
+                uint32_t w[4][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 u = T::unpack(braw[i].x), z = T::unpack(braw[i].y);
-                    w[i][0] = __float_as_uint(u.x); w[i][1] = __float_as_uint(u.y); w[i][2] = __float_as_uint(z.x); w[i][3] = __float_as_uint(z.y);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j + e >= rank) w[i][e] = 0u;       // nor what B has there
-                }
+                for (int i = 0; i < 4; ++i) { w[i][0] = braw[i].x & m0; w[i][1] = braw[i].y & m1; }
                 const bool last = 16 * rt + 16 >= rank;
                 if (!last || c + AD_WARPS < end) load_b(braw, last ? c + AD_WARPS : c, last ? 0 : rt + 1);
-                // two eights of tokens at a time, and no product right behind another one into the same accumulator
+                uint4 x[4];
+                uint2 z[4];
 #pragma unroll
-                for (int n2 = 0; n2 < 4; n2 += 2) {
-                    uint32_t hi[2][4], lo[2][4];
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const uint8_t* src = hs + ((8 * (n2 + nt) + g) * C::LDH + j) * 8;
-                        const uint4 u = *reinterpret_cast<const uint4*>(src), v = *reinterpret_cast<const uint4*>(src + 16);
-                        hi[nt][0] = u.x; lo[nt][0] = u.y; hi[nt][1] = u.z; lo[nt][1] = u.w;
-                        hi[nt][2] = v.x; lo[nt][2] = v.y; hi[nt][3] = v.z; lo[nt][3] = v.w;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; k += 2)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-#pragma unroll
-                            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                                for (int i = 0; i < 2; ++i) {
-                                    const uint32_t(&x)[4] = e ? hi[nt] : lo[nt];
-                                    mma_tf32(acc[i][n2 + nt], w[2 * i][k], w[2 * i + 1][k], w[2 * i][k + 1], w[2 * i + 1][k + 1], x[k], x[k + 1]);
-                                }
+                for (int nt = 0; nt < 4; ++nt) {
+                    x[nt] = *reinterpret_cast<const uint4*>(hs + (8 * nt + g) * C::LDH + 4 * j);
+                    if constexpr (T::PARTS == 3) z[nt] = *reinterpret_cast<const uint2*>(hs + AD_TOK * C::LDH + (8 * nt + g) * C::LDH3 + 2 * j);
                 }
+                // the smallest part first; no product right behind another one into the same accumulator
+#pragma unroll
+                for (int k = T::PARTS - 1; k >= 0; --k)
+#pragma unroll
+                    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            T::mma(acc[i][nt], w[2 * i][0], w[2 * i + 1][0], w[2 * i][1], w[2 * i + 1][1], k == 2 ? z[nt].x : k ? x[nt].z : x[nt].x,
+                                   k == 2 ? z[nt].y : k ? x[nt].w : x[nt].y);
             }
+            if constexpr (T::PARTS == 2)
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt) {
+                    const float2 u = *reinterpret_cast<const float2*>(hs + AD_TOK * (C::LDH + C::LDH3) + 4 * (8 * nt + 2 * t));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) { acc[i][nt][0] *= u.x; acc[i][nt][1] *= u.y; acc[i][nt][2] *= u.x; acc[i][nt][3] *= u.y; }
+                }
             if (!mine) continue;
             float* yrow = p.Y + n0 * p.ldy + P.row0 + row;
 #pragma unroll

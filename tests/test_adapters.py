@@ -2,9 +2,9 @@
 
 Where everything is a small whole number nothing is rounded, and the results have to be equal. Elsewhere the bound is the sum of the
 roundings: a group's 128 exact products are added in eight instructions of sixteen (four roundings of 2^-23 each allowed, the tensor core
-truncates), then a multiply-add for each group and three more operations; H as two tf32 numbers keeps 2^-22 of it; the second product is one
-instruction for eight ranks and each part, four roundings of 2^-23 each again; the addition into Y is one rounding. Each is relative to the sum of
-the absolute values of what is added."""
+truncates), then a multiply-add for each group and three more operations; H in parts (two of tf32 or fp16, three of bf16) keeps 2^-22 of it at
+least; the second product is one instruction for eight ranks and each part at most, four roundings of 2^-23 each again; the addition into Y is one rounding. Each is
+relative to the sum of the absolute values of what is added."""
 import importlib
 
 import numpy as np
@@ -88,7 +88,11 @@ def _random_segments(T, nseg, n, seed):
 # (tokens, segments, K, rank, adapters, parts)
 CASES = [(1, 1, 2048, 8, 3, [(0, 2048)]), (1, 1, 128, 8, 1, [(0, 4)]), (7, 7, 256, 16, 9, [(4, 36)]), (32, 1, 2048, 16, 2, [(0, 2048)]), (33, 1, 1152, 24, 2, [(0, 512)]),
          (31, 2, 128, 128, 2, [(0, 132)]), (100, 5, 384, 40, 4, [(8, 260)]), (64, 64, 512, 32, 5, [(0, 512)]), (257, 3, 2176, 64, 3, [(0, 1024), (1280, 256)]),
-         (300, 300, 256, 8, 7, [(0, 64), (64, 128), (192, 32), (240, 4)]), (515, 20, 2048, 72, 6, [(0, 256)]), (90, 700, 128, 8, 4, [(0, 96)]), (40, 2, 4224, 128, 2, [(0, 2048)])]
+         (300, 300, 256, 8, 7, [(0, 64), (64, 128), (192, 32), (240, 4)]), (515, 20, 2048, 72, 6, [(0, 256)]), (90, 700, 128, 8, 4, [(0, 96)]), (40, 2, 4224, 128, 2, [(0, 2048)]),
+         # many tiles: clusters of four, two and one for each of the kernels
+         (1700, 3, 256, 16, 2, [(0, 96)]), (3001, 40, 384, 16, 3, [(0, 64)]), (9600, 5, 128, 8, 2, [(0, 36)]), (1300, 3, 384, 24, 2, [(0, 68)]), (4900, 7, 128, 32, 2, [(0, 32)]),
+         (10000, 2, 128, 32, 2, [(0, 32)]), (900, 9, 384, 48, 3, [(0, 300)]), (2500, 1, 256, 40, 1, [(0, 132)]), (4800, 3, 128, 64, 2, [(0, 260)]), (1000, 2, 256, 96, 2, [(0, 140)]),
+         (1500, 1, 128, 128, 1, [(0, 132)]), (5000, 2, 128, 72, 2, [(0, 132)])]
 
 
 @pytest.mark.gpu
@@ -144,6 +148,49 @@ def test_adapters_leave_alone_what_is_not_theirs(api, orc, dtype):
     got = _run(api, orc, q, s, Y, ab, parts, [0, T], [0], None, [2 ** 31 - 1] * n)             # a rank beyond the pool's is the pool's
     want, bound = _plain(q, s, Y, ab, parts, [(0, T, 0)], None, None)
     assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rank", [16, 32, 64])
+def test_adapters_of_any_magnitude(api, orc, rank, dtype):
+    """Ranks whose parts of H differ by many powers of two, tokens of all sizes and zeros: each within its own bound."""
+    T, K, n, parts = 48, 256, 2, [(0, 64)]
+    q, s, Y, ab = _case(T, K, rank, n, parts, dtype, 7)
+    s *= (2.0 ** np.linspace(-40, 40, T))[:, None].astype(np.float32)
+    q[5] = 0
+    s[6] = 0
+    A, B = ab[0]
+    A *= (2.0 ** torch.linspace(-8, 8, rank))[None, :, None].to(dtype)
+    want, bound = _plain(q, s, Y, ab, parts, [(0, T, 1)], None, None)
+    got = _run(api, orc, q, s, Y, ab, parts, [0, T], [1])
+    assert (np.abs(got - want) <= bound).all() and np.array_equal(got[5:7], Y[5:7])
+
+
+@pytest.mark.gpu
+def test_adapters_far_into_the_memory(api, orc):
+    """Elements of Y, and of a pool's A, whose index does not fit 31 bits."""
+    g = torch.Generator(device="cuda"); g.manual_seed(3)
+    T, K, rows, rank = 2_200_000, 128, 1024, 8
+    Y = torch.zeros((T, rows), device="cuda")
+    q = torch.randint(-9, 10, (T, K), generator=g, device="cuda", dtype=torch.int8)
+    s = torch.ones((T, 1), device="cuda")
+    A, B = torch.randint(-2, 3, (2, rank, K), generator=g, device="cuda").half(), torch.randint(-2, 3, (2, rows, rank), generator=g, device="cuda").half()
+    first = torch.tensor([0, T - 40, T - 3], dtype=torch.int32, device="cuda")
+    api.adapters_w4a8(api.adapter_pools([api.AdapterPool(A, B)]), q, s, Y, first, torch.tensor([-1, 1], dtype=torch.int32, device="cuda"))
+    x = q[T - 40:].float()[:, torch.from_numpy(_frag(orc, K)).cuda()]
+    want = x @ A[1].float().t() @ B[1].float().t()
+    want[-3:] = 0
+    assert torch.equal(Y[T - 40:], want) and not bool(Y[T - 80:T - 40].any()) and not bool(Y[:1000].any())
+    del Y, q
+    n, K, rank = 1100, 16384, 128
+    A = torch.zeros((n, rank, K), dtype=torch.half, device="cuda")
+    A[n - 1] = torch.randint(-1, 2, (rank, K), generator=g, device="cuda").half()
+    B = torch.ones((n, 8, rank), dtype=torch.half, device="cuda")
+    q, s, Y = torch.randint(-1, 2, (3, K), generator=g, device="cuda", dtype=torch.int8), torch.ones((3, K // 128), device="cuda"), torch.zeros((3, 8), device="cuda")
+    api.adapters_w4a8(api.adapter_pools([api.AdapterPool(A, B)]), q, s, Y, torch.tensor([0, 3], dtype=torch.int32, device="cuda"), torch.tensor([n - 1], dtype=torch.int32, device="cuda"))
+    want = (q.float()[:, torch.from_numpy(_frag(orc, K)).cuda()] @ A[n - 1].float().t()).sum(1, keepdim=True).expand(3, 8)
+    assert torch.equal(Y, want) and bool(Y.any())
 
 
 @pytest.mark.gpu

@@ -165,6 +165,23 @@ def test_norm_takes_columns_of_one_matrix(api, orc):
 
 
 @pytest.mark.gpu
+def test_norm_far_into_the_memory(api):
+    """Rows whose values lie beyond 31 bits of index, in the residual, the codes and the 16-bit copy: what a call on these rows alone gives."""
+    T, K = 1_060_000, 2048
+    x = torch.full((T, K), 0.5, device="cuda")
+    x[-50:] = torch.randn((50, K), device="cuda")
+    d, gain = torch.ones((T, K), dtype=torch.half, device="cuda"), torch.ones(K, device="cuda")
+    new = lambda n: (torch.zeros((n, K), dtype=torch.int8, device="cuda"), torch.zeros((n, K // 128), device="cuda"), torch.zeros((n, K // 128), dtype=torch.int32, device="cuda"))
+    tail, outs, y = x[-50:].clone(), new(T), torch.zeros((T, K), dtype=torch.half, device="cuda")
+    api.add_norm_q8(x, gain, 1e-6, *outs, delta=d, y=y)
+    few, yf = new(50), torch.zeros((50, K), dtype=torch.half, device="cuda")
+    api.add_norm_q8(tail, gain, 1e-6, *few, delta=d[:50], y=yf)
+    assert torch.equal(x[-50:], tail) and torch.equal(outs[0][-50:], few[0]) and torch.equal(outs[2][-50:], few[2])
+    assert torch.allclose(outs[1][-50:], few[1], rtol=1e-6, atol=0) and torch.allclose(y[-50:].float(), yf.float(), rtol=2.0 ** -10, atol=0)
+    assert bool((x[:100] == 1.5).all()) and bool((outs[0][:100] == 127).all()) and bool((y[:100] == 1).all())
+
+
+@pytest.mark.gpu
 def test_norm_feeds_the_projection(api, orc, pkg):
     x, d, gain = _inputs(70, 2048, torch.float16, 31)
     got = _run(api, x, d, gain, 1e-6)[1]
