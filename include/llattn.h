@@ -115,7 +115,7 @@ int llattn_dense_w4a8(const void* W, const int8_t* q, const float* s, const int3
 #define LLATTN_DENSE_TCGEN05 2 /* 128 rows per CTA, tcgen05 */
 int llattn_dense_preview(int rows, int K, int ntokens, int num_sms, int* kernel, int* tokens_per_cta);
 
-/* Reads (and clears) the current device's word for llattn_dense_w4a8 calls without one of their own; synchronises `stream`.
+/* Reads (and clears) the current device's word for llattn_dense_w4a8 calls without one of their own, and for llattn_adapters_w4a8; synchronises `stream`.
  * LLATTN_EDEVICE and the bits in *code when a wait of any such call on the device ran out since the word was last read: call
  * it where the results of a step are read, behind the work of every stream that ran such calls. No counterpart in the
  * reference, whose kernels have no waits that can fail. */
@@ -158,10 +158,13 @@ typedef struct llattn_adapter_pool {
 /* The tokens [seg_first[i], seg_first[i + 1]) belong to segment i, whose adapter is seg_adapter[i] in every pool (both device arrays, nseg + 1
  * and nseg long, bounds ascending; -1, or an index that the pool does not have: none). For a token n of a segment with adapter a, and every pool:
  *   Y[n][row0 + i] += scale[a] * sum_j B[a][i][j] * sum_k A[a][j][k] * s[n][k / 128] * q[n][k]
- * from the activations (q, s) that the projection itself reads, added in fp32; the order of the sums, and so the bits, depends on the sizes only.
- * Y has ldy values a row (a multiple of 4, at least row0 + rows); tokens outside the segments, and of a segment without an adapter, keep
- * theirs. `pools` is a host array of 1 to 4 pools of one type whose rows do not overlap (the q, k and v parts of one projection, say), read
- * during the call; what is on the device may change between replays of a captured call. */
+ * from the activations (q, s) that the projection itself reads. All sums are fp32, and 22 bits of the inner one go into the outer one; the result is
+ * added to Y in the memory, rounded once (numbers below 2^-126 count as zero there; an infinite inner sum makes NaN). The order of the sums, and so
+ * the bits, depends on ntokens, nseg, npools, K and the pools' sizes only. Y has ldy values a row (a multiple of 4, at least row0 + rows); tokens
+ * outside the segments, and of a segment without an adapter, keep theirs. q and Y are 16-byte aligned. `pools` is a host array of 1 to 4 pools
+ * of one type whose rows do not overlap (the q, k and v parts of one projection, say), read during the call; what is on the device may change
+ * between replays of a captured call. At most 65,536 segments. A wait for another CTA or for the tensor cores that runs out is reported where those
+ * of the projection are, see llattn_dense_status: some of Y then has its adapters added and some has not. */
 int llattn_adapters_w4a8(const llattn_adapter_pool* pools, int npools, const int8_t* q, const float* s, float* Y, int64_t ldy, int ntokens,
                          int K, const int32_t* seg_first, const int32_t* seg_adapter, int nseg, void* stream);
 

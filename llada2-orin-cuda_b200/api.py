@@ -363,6 +363,8 @@ def _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v):
 def qk_norm_rope_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream=None) -> None:
     """qk_norm_rope with several position axes: pos int32 [axes][T], axis_of the axis of each of the 32 frequencies (host; see rope_axes)."""
     T, args = _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v)
+    if T == 0:                               # (an empty tensor has no address)
+        return
     _check(lib().llattn_qk_norm_rope_axes(*args, T, _stream(stream)))
 
 
@@ -376,6 +378,8 @@ def qkv_prepare_commit_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v,
         raise ValueError("a prefill pass commits whole 32-token blocks")
     if pages is None and cache.numel() < NKV * max_blocks * KV_BLOCK_BYTES:
         raise ValueError("the cache holds fewer than max_blocks blocks")
+    if T == 0:
+        return
     _check(lib().llattn_qkv_prepare_commit_axes(*args, nb, _flat(cache, torch.uint8, cache.numel(), dev, "cache"),
                                                 None if pages is None else _flat(pages, torch.int32, nb * NKV, dev, "pages"), max_blocks, blk, _stream(stream)))
 
@@ -401,6 +405,8 @@ def add_norm_q8(x, gain, eps, q=None, s=None, qsum=None, delta=None, y=None, str
         raise ValueError("q, s and qsum go together")
     if y is not None:
         yp, ytype = _flat(y, y.dtype, T * K, dev, "y"), types.get(y.dtype, -1)
+    if T == 0:                               # (an empty tensor has no address)
+        return
     _check(lib().llattn_add_norm_q8(xp, ldx, dp, dtype, ldd, _flat(gain, torch.float32, K, dev, "gain"), eps, qp, sp, sump, yp, ytype, T, K, _stream(stream)))
 
 
@@ -455,6 +461,8 @@ def adapters_w4a8(pools: AdapterPools, q, s, Y, seg_first, seg_adapter, stream=N
     if pools._rows > width or pools.device != dev:
         raise ValueError(f"the pools' rows reach to {pools._rows} of {width}, on cuda:{pools.device}; the current device is cuda:{dev}")
     yp, ldy = _rows(Y, f32, T, width, dev, "Y")
+    if T == 0 or nseg == 0:                  # (an empty tensor has no address)
+        return
     _check(lib().llattn_adapters_w4a8(pools._c, len(pools._c), _flat(q, torch.int8, T * K, dev, "q"), _flat(s, f32, T * (K // 128), dev, "s"), yp, ldy, T, K,
                                       _flat(seg_first, i32, nseg + 1, dev, "seg_first"), _flat(seg_adapter, i32, nseg, dev, "seg_adapter"), nseg, _stream(stream)))
 

@@ -119,6 +119,8 @@ template <int RT> struct AdapterTile {
     static constexpr int AREA = H_AT + (WIDE ? R / 32 * HBLOCK : TOK * (LDH + LDH3 + 4));
     static constexpr int HEAD = WIDE ? 1024 : 64;
     static constexpr int bytes(int ctas) { return HEAD + (ctas - 1) * SLOT + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
+    static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : 4;        // CTAs of a cluster
+    static_assert(bytes(MOST) <= 227 * 1024, "shared memory of the largest cluster");
 };
 
 // Four neighbouring values added in L2: Y need not come here. Every value of a call is added to once, so no order matters; an fp32 addition rounded to
@@ -567,7 +569,7 @@ namespace {
 // 24.4 / 21.4 / 27.7 / -; rank 64, 8 segments of 128 tokens 35.5 / 20.7 / 14.2 / 31, 4096 tokens 35.8 / 31.1 / 37.0 / -.
 template <int RT> int adapter_parts(long long ntokens, long long nseg, int npools, int sms) {
     const long long tiles = std::max(std::min(nseg, ntokens), (ntokens + llattn::AD_TOK - 1) / llattn::AD_TOK) * npools;
-    int parts = 8;
+    int parts = llattn::AdapterTile<RT>::MOST;
     while (parts > 1 && parts * tiles > (llattn::AdapterTile<RT>::bytes(parts) <= 113 * 1024 ? 2 : 1) * sms) parts /= 2;
     return parts;
 }
@@ -575,15 +577,14 @@ template <int RT> int adapter_parts(long long ntokens, long long nseg, int npool
 template <typename T, int RT>
 int launch_adapters(llattn::AdapterParams& p, int npools, int sms, cudaStream_t stream) {
     using namespace llattn;
-    static std::once_flag once[64];
+    static std::atomic<bool> ready[64];
     auto* kernel = adapters_kernel<T, RT>;
-    constexpr int most = AdapterTile<RT>::bytes(8);
-    static_assert(most <= 227 * 1024, "shared memory of the largest cluster");
+    constexpr int most = AdapterTile<RT>::bytes(AdapterTile<RT>::MOST);
     int dev = 0;
     CU(cudaGetDevice(&dev));
-    if (most > 48 * 1024) {
-        if (dev < 0 || dev >= 64) CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-        else std::call_once(once[dev], [&] { cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most); });
+    if (most > 48 * 1024 && (dev >= 64 || !ready[dev])) {
+        CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        if (dev < 64) ready[dev] = true;
     }
     p.parts = adapter_parts<RT>(p.ntokens, p.nseg, npools, sms);
     // no more tiles than this, however the segments cut the tokens: each has at most one that is not full

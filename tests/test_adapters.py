@@ -6,6 +6,9 @@ truncates), then a multiply-add for each group and three more operations; H in p
 least; the second product is one instruction for eight ranks and each part at most, four roundings of 2^-23 each again; the addition into Y is one rounding. Each is
 relative to the sum of the absolute values of what is added."""
 import importlib
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -200,6 +203,49 @@ def test_adapters_of_nan_activations_are_nan(api, orc):
     s[3, 1] = np.nan
     got = _run(api, orc, q, s, Y, ab, parts, [0, T], [1])
     assert np.isnan(got[3, :64]).all() and np.isfinite(np.delete(got, 3, 0)).all() and np.array_equal(got[3, 64:], Y[3, 64:])
+
+
+@pytest.mark.gpu
+def test_adapters_first_call_under_capture(pkg):
+    """A process whose first call of a kernel is captured: nothing that a call sets up once may disturb the capture."""
+    code = f"""
+import importlib, torch
+api = importlib.import_module({pkg.__name__!r} + ".api")
+z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device="cuda")
+T = 40
+q, s, Y, first, adapter = torch.ones((T, 256), dtype=torch.int8, device="cuda"), torch.ones((T, 2), device="cuda"), z(T, 64), torch.tensor([0, T], dtype=torch.int32, device="cuda"), z(1, dtype=torch.int32)
+for dtype in (torch.half, torch.bfloat16):
+    for rank in (8, 32, 64, 128):
+        pools = api.adapter_pools([api.AdapterPool(torch.ones((1, rank, 256), dtype=dtype, device="cuda"), torch.ones((1, 64, rank), dtype=dtype, device="cuda"))])
+        x, n8, ns, nsum = z(T, 256), z(T, 256, dtype=torch.int8), z(T, 2), z(T, 2, dtype=torch.int32)
+        graph = torch.cuda.CUDAGraph()
+        Y.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            api.adapters_w4a8(pools, q, s, Y, first, adapter)
+            api.add_norm_q8(x, torch.ones(256, device="cuda"), 1e-6, n8, ns, nsum)
+        assert not bool(Y.any())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((Y == 256 * rank).all()), (dtype, rank)
+assert api.dense_status() == 0
+print("done")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-1500:]
+
+
+@pytest.mark.gpu
+def test_nothing_to_do(api):
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device="cuda")
+    i32, pools = torch.int32, api.adapter_pools([api.AdapterPool(z(1, 8, 128, dtype=F16), z(1, 4, 8, dtype=F16))])
+    api.adapters_w4a8(pools, z(0, 128, dtype=torch.int8), z(0, 1), z(0, 4), z(2, dtype=i32), z(1, dtype=i32))
+    api.adapters_w4a8(pools, z(3, 128, dtype=torch.int8), z(3, 1), z(3, 4), z(1, dtype=i32), z(0, dtype=i32))
+    api.add_norm_q8(z(0, 128), z(128), 1e-6, z(0, 128, dtype=torch.int8), z(0, 1), z(0, 1, dtype=i32))
+    freq, axes = torch.from_numpy(api.inv_freq()).cuda(), api.rope_axes([16, 16])
+    out = [z(0, n, 128, dtype=F16) for n in (16, 4, 4)]
+    api.qk_norm_rope_axes(z(0, 3072), z(2, 0, dtype=i32), axes, z(128), z(128), 1e-6, freq, *out)
+    api.qkv_prepare_commit_axes(z(0, 3072), z(2, 0, dtype=i32), axes, z(128), z(128), 1e-6, freq, *out, z(4, 1, 4736, dtype=torch.uint8), max_blocks=1)
 
 
 def _args(api, **changed):
