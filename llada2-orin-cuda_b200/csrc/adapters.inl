@@ -5,12 +5,26 @@
 //   Y[n][row0 + i] += sum_j H[n][j] * B_a[i][j]
 // from the int8 activations that the projection itself reads (codes in fragment order, one scale for each group of 128).
 //
-// A CTA takes up to 32 tokens of one segment and a part of the rows. First product: the codes are exact in 16 bits, so mma.sync multiplies them
-// with A as it is, and each group's sum takes its scale in fp32: nothing is rounded but the fp32 sums. A lane's word of the fragment order is
-// four neighbouring values of a run of sixteen; the four K slots of a lane in an m16n8k16 are given to just these, and A is read to match, eight
-// bytes a lane. Second product: H is two tf32 numbers, value and remainder (22 bits; one alone would leave 2^-11 of the adapter's
-// part, and bf16 pairs 2^-17), B is exact in tf32. A warp takes 32 rows, four for each of its eight row lanes, so that a token's 32 values of
-// Y are one 128-byte line and every access to Y is 16 bytes a lane.
+// A cluster takes up to 32 tokens of one segment. Each of its CTAs has a part of the groups in the first product and a part of the rows in the second;
+// in between it stores its sums of H into the others' shared memory (st.async, counted in on a barrier there), and each adds all of them up in
+// the CTAs' order.
+//
+// First product: the codes are exact in 16 bits, so mma.sync multiplies them with A as it is, and each group's sum takes its scale in fp32: nothing is
+// rounded but the fp32 sums. A lane's word of the fragment order is four neighbouring values of a run of sixteen; the four K slots of a lane
+// in an m16n8k16 are given to just these, and A is read to match, eight bytes a lane. Groups of A, codes and scales come through cp.async, two to four
+// ahead.
+//
+// Second product: B is multiplied as it is, too, with H in parts: two of fp16 (22 bits, behind a power of two that brings the token's largest to 2^13)
+// or three of bf16 (24 bits). One part alone would leave 2^-11 or 2^-8 of the adapter's contribution, two of bf16 2^-17 = 8e-6, an order above the
+// rest of the sums' error. Up to 32 ranks with mma.sync, a warp for 32 rows: four for each of its eight row lanes, so that a token's 32 values
+// of Y are one 128-byte line and a lane adds 16 bytes of it. More ranks on tcgen05: 128 rows of B as the A operand, 64 or 96 columns of all parts of the
+// tokens' H as the B operand, B copied into the swizzled tile in an order of rows that gives a thread four neighbouring ones from tensor memory.
+// Y is added to by vector reductions in L2 and never comes to an SM: loading and storing it instead took 22 us in the place of 13 for 64 segments of 32 tokens.
+//
+// What bounds it: one token 4.9 us, a chain of launch, segment, operands, the cluster's exchange (1.2 us) and B. A full batch (64 segments of 32 tokens,
+// adapters of rank 16) 13.0 us = 3.5 TB/s cold and 10.0 warm, of which 9.1 without the additions to Y: reading, computing and adding
+// overlap only across CTAs, and the chip holds all of them at once. 4096 tokens of rank 64 28.7 us, issue slots and shared memory of the first product
+// (45 %), the second product's tiles (the rest); with tf32 pairs on mma.sync 45, with one CTA a tile and every operand from memory 205.
 #pragma once
 
 namespace llattn {
@@ -48,7 +62,7 @@ struct AdapterF16 {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
-    static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const half2*>(&w)); }
+    static constexpr uint32_t IDESC = 0;       // operand types of kind::f16
     static constexpr int PARTS = 2;            // of H, in fp16: 22 bits of a value, the largest of a token brought to 2^13
     static __device__ __forceinline__ uint32_t part(float& a, float& b) {      // two values rounded, what is left of them in their place
         const half2 x = __floats2half2_rn(a, b);
@@ -70,7 +84,7 @@ struct AdapterBF16 {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
-    static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    static constexpr uint32_t IDESC = 1u << 7 | 1u << 10;
     static constexpr int PARTS = 3;            // of H, in bf16: 24 bits, and no range to be kept
     static __device__ __forceinline__ uint32_t part(float& a, float& b) {
         const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
@@ -78,28 +92,25 @@ struct AdapterBF16 {
         return *reinterpret_cast<const uint32_t*>(&x);
     }
 };
-// 32 ranks: four K-steps of kind::tf32 over 128-byte-swizzle tiles (A: 128 rows of B, B: the tokens' H). One elected lane issues.
-__device__ __forceinline__ void mma_tf32_block_warp(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate_first) {
+// 64 ranks: four K-steps of kind::f16 over 128-byte-swizzle tiles (A: 128 rows of B, B: the parts of the tokens' H). One elected lane issues.
+__device__ __forceinline__ void mma_f16_block_warp(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate_first) {
     asm volatile(
         "{\n\t.reg .pred pe, pf, pt;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
         "elect.sync _|pe, 0xffffffff;\n\t"
         "setp.ne.b32 pf, %5, 0;\n\t setp.eq.b32 pt, 0, 0;\n\t"
         "mov.b64 da, {%1, %3};\n\t mov.b64 db, {%2, %3};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, pf;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, pf;\n\t"
         "add.u32 x, %1, 2;\n\t add.u32 y, %2, 2;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, pt;\n\t"
         "add.u32 x, %1, 4;\n\t add.u32 y, %2, 4;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, pt;\n\t"
         "add.u32 x, %1, 6;\n\t add.u32 y, %2, 6;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, pt;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, pt;\n\t"
         "}\n" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate_first) : "memory");
 }
-// kind::tf32 instruction descriptor: fp32 accumulator, both operands tf32 and K-major.
-__host__ __device__ constexpr uint32_t idesc_tf32(int M, int N) { return (1u << 4) | (2u << 7) | (2u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24); }
-__device__ __forceinline__ uint32_t to_tf32(float x) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
+// Sixteen bytes of which the first `bytes` are copied and the others become zeros.
+__device__ __forceinline__ void cp_async16_some(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // A CTA of RT sixteens of ranks and 32 tokens: its warps' shares and its shared memory.
@@ -109,14 +120,14 @@ template <int RT> struct AdapterTile {
     static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WK = AD_WARPS / WR;
     // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
     static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : RT > 1 ? 3 : 5;
-    // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], or the tensor cores' tile of B, and H: for few ranks as parts
-    // of 16 bits, the first two [TOK] rows LDH bytes apart, the third, and a power of two for each token, else as the tensor cores' tiles of both parts. In front of all a slot [TOK][R] for the sums of each other CTA of
-    // the cluster.
+    // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], and H in parts of 16 bits. For few ranks the first two parts [TOK]
+    // rows LDH bytes apart, and the third; else the tensor cores' tiles, 64 ranks a block, and behind them tiles of 128 rows of B. A power of two for each
+    // token. In front of all a slot [TOK][R] for the sums of each other CTA of the cluster.
     static constexpr bool WIDE = RT >= 4;
     static constexpr int LDP = R + 4, LDH = 4 * R + (RT == 2 ? 64 : 0), LDH3 = LDH / 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
-    static constexpr int WBLOCK = 128 * 128, HBLOCK = 2 * TOK * 128;       // 32 ranks of 128 rows, of the tokens' values and of their remainders
-    static constexpr int H_AT = !WIDE ? SUMS : (SUMS > R / 32 * WBLOCK ? (SUMS + 1023) / 1024 * 1024 : R / 32 * WBLOCK);
-    static constexpr int AREA = H_AT + (WIDE ? R / 32 * HBLOCK : TOK * (LDH + LDH3 + 4));
+    static constexpr int BLOCKS = (R + 63) / 64, HBLOCK = 3 * TOK * 128, WBLOCK = 128 * 128, WTILE = BLOCKS * WBLOCK, WTILES = RT > 4 ? 1 : 2;
+    static constexpr int H_AT = WIDE ? (SUMS + 1023) / 1024 * 1024 : SUMS, W_AT = H_AT + BLOCKS * HBLOCK;
+    static constexpr int UP_AT = WIDE ? W_AT + WTILES * WTILE : H_AT + TOK * (LDH + LDH3), AREA = UP_AT + TOK * 4;
     static constexpr int HEAD = WIDE ? 1024 : 64;
     static constexpr int bytes(int ctas) { return HEAD + (ctas - 1) * SLOT + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
     static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : 4;        // CTAs of a cluster
@@ -248,7 +259,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
     };
     for (int i = 0; i < C::STAGES - 1; ++i) fetch(i);
     if constexpr (C::WIDE)
-        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), 2 * AD_TOK); ptx::tmem_relinquish(); }
+        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), 128); ptx::tmem_relinquish(); }
     const int rank_there = P.ranks ? __ldg(P.ranks + a) : P.rank;  // looked at when the sums are there: a wait for it here would hold up what follows
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
     // ---- this CTA's rows of B are wanted when H is done: into L2, and a small rank's first ones into registers
@@ -322,6 +333,21 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
     cp_async_wait<0>();
     __syncthreads();                           // the stages are done with
     const int rank = min(max(rank_there, 0), P.rank);
+    // 128 rows of B as the tensor cores read them: row 4 g + i of 32 is the tile's g + 8 i, a thread then gets four neighbouring rows from tensor memory.
+    // Behind the rank, whatever B has there, and behind P's rows: zeros.
+    auto fetch_b = [&](int c) {
+        if (c < end)
+#pragma unroll
+            for (int m = 0; m < 128 * C::R / 8; m += AD_THREADS) {
+                const int r = (m + tid) / (C::R / 8), j = (m + tid) % (C::R / 8) * 8, row = 128 * c + r, at = r / 32 * 32 + r / 4 % 8 + r % 4 * 8;
+                const int bytes = row < P.rows ? min(max(rank - j, 0), 8) * 2 : 0;
+                cp_async16_some(area_s + C::W_AT + (c - first) % C::WTILES * C::WTILE + j / 64 * C::WBLOCK + at * 128 + ((j % 64 / 8 ^ (at & 7)) << 4),
+                                bytes ? B + size_t(row) * P.rank + j : B, bytes);
+            }
+        cp_async_commit();
+    };
+    if constexpr (C::WIDE)
+        for (int c = first; c < first + C::WTILES; ++c) fetch_b(c);
     float* sums = reinterpret_cast<float*>(area);
 #pragma unroll
     for (int r = 0; r < C::RW; ++r)
@@ -370,120 +396,96 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = j + e < rank ? v[e] * scale : 0.f;      // what A has behind the rank, whatever it is, does not count
+            if constexpr (T::PARTS == 2) {                         // the token's ranks are with R / 4 neighbouring lanes
+                float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+                for (int o = 1; o < C::R / 4; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int e = most < INFINITY ? max(int(__float_as_uint(most) >> 23) - 127, -100) : 13;
+                const float up = __uint_as_float(uint32_t(127 + 13 - e) << 23);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] *= up;
+                if (j == 0) reinterpret_cast<float*>(area + C::UP_AT)[n] = __uint_as_float(uint32_t(127 - 13 + e) << 23);
+            }
+            uint32_t w[T::PARTS][2];
+#pragma unroll
+            for (int k = 0; k < T::PARTS; ++k) { w[k][0] = T::part(x[0], x[1]); w[k][1] = T::part(x[2], x[3]); }
             if constexpr (C::WIDE) {
-                uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    hi[e] = to_tf32(x[e]);
-                    lo[e] = to_tf32(x[e] - __uint_as_float(hi[e]));
-                }
-                uint8_t* to = hs + j / 32 * C::HBLOCK + n * 128 + ((j % 32 / 4 ^ (n & 7)) << 4);
-                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(to + AD_TOK * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                for (int k = 0; k < T::PARTS; ++k)
+                    *reinterpret_cast<uint2*>(hs + j / 64 * C::HBLOCK + (AD_TOK * k + n) * 128 + ((j % 64 / 8 ^ (n & 7)) << 4) + j % 8 * 2) = make_uint2(w[k][0], w[k][1]);
             } else {
-                if constexpr (T::PARTS == 2) {                     // the token's ranks are with R / 4 neighbouring lanes
-                    float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-                    for (int o = 1; o < C::R / 4; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    const int e = most < INFINITY ? max(int(__float_as_uint(most) >> 23) - 127, -100) : 13;
-                    const float up = __uint_as_float(uint32_t(127 + 13 - e) << 23);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) x[k] *= up;
-                    if (j == 0) reinterpret_cast<float*>(hs + AD_TOK * (C::LDH + C::LDH3))[n] = __uint_as_float(uint32_t(127 - 13 + e) << 23);
-                }
-                uint32_t w[T::PARTS][2];
-#pragma unroll
-                for (int k = 0; k < T::PARTS; ++k) { w[k][0] = T::part(x[0], x[1]); w[k][1] = T::part(x[2], x[3]); }
                 *reinterpret_cast<uint4*>(hs + n * C::LDH + 4 * j) = make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
                 if constexpr (T::PARTS == 3) *reinterpret_cast<uint2*>(hs + AD_TOK * C::LDH + n * C::LDH3 + 2 * j) = make_uint2(w[2][0], w[2][1]);
             }
         }
     }
+    if constexpr (C::WIDE) ptx::fence_proxy_async_smem();
     ok = __syncthreads_and(ok);                // H is there; where sums are missing this CTA leaves Y as it is
     if constexpr (C::WIDE) {
-        // ---- Y, 128 rows at a time on tcgen05: B as tf32 into its tile, both parts of H times it into tensor memory, from there a thread to a row
+        // ---- Y, 128 rows at a time on tcgen05: a tile of B times all parts of H beside one another into tensor memory
         ptx::tc_fence_after();
-        const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 20), wtile = area_s;
-        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = idesc_tf32(128, 2 * AD_TOK);
-        constexpr int CH = C::R / 8, LOADS = 128 * CH / AD_THREADS, HALF = AD_TOK / 2;
-        uint4 wr16[LOADS];
-        auto load_w = [&](int c) {
-#pragma unroll
-            for (int m = 0; m < LOADS; ++m) {
-                const int k = tid + m * AD_THREADS, row = 128 * c + k / CH, j = k % CH * 8;
-                wr16[m] = make_uint4(0u, 0u, 0u, 0u);
-                if (c < end && row < P.rows && j < rank) wr16[m] = __ldg(reinterpret_cast<const uint4*>(B + size_t(row) * P.rank + j));
-            }
-        };
-        if (rank == 0) ok = false;
+        const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 20);
+        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = ptx::idesc_f16(128, T::PARTS * AD_TOK, false, false) | T::IDESC;
+        constexpr int COLS = AD_TOK / 2;       // of a warp: a quarter of the rows, half of the tokens
         const bool wanted = rank != 0;
+        const int nw = COLS * (warp >> 2);
+        float2 down[COLS / 8];
+#pragma unroll
+        for (int i = 0; i < COLS / 8; ++i) down[i] = T::PARTS == 2 ? *reinterpret_cast<const float2*>(area + C::UP_AT + 4 * (nw + 8 * i + 2 * t)) : make_float2(1.f, 1.f);
         int issued = 0;
-        if (ok) load_w(first);
+        ok = ok && wanted;
 #pragma unroll 1
         for (int c = first; c < end; ++c) {
-            if (ok) {
-#pragma unroll
-                for (int m = 0; m < LOADS; ++m) {
-                    const int k = tid + m * AD_THREADS, r = k / CH, j = k % CH * 8;
-                    const uint32_t raw[4] = {wr16[m].x, wr16[m].y, wr16[m].z, wr16[m].w};
-                    float f[8];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { const float2 u = T::unpack(raw[e]); f[2 * e] = u.x; f[2 * e + 1] = u.y; }
-                    if (j + 8 > rank)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (j + e >= rank) f[e] = 0.f;                     // nor what B has there
-                    const int g8 = r / 4 % 8;      // row 4 g + i of 32 is the tile's g + 8 i: a thread then gets four neighbouring rows from tensor memory
-                    uint8_t* to = area + j / 32 * C::WBLOCK + (r / 32 * 32 + g8 + r % 4 * 8) * 128;
-                    // of the two halves the odd blocks' lanes store the second first: else they would meet the even ones' in the same banks
-                    const bool odd = j / 32 & 1;
-                    const float4 lo = make_float4(f[0], f[1], f[2], f[3]), hi = make_float4(f[4], f[5], f[6], f[7]);
-                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 + odd ^ g8) << 4)) = odd ? hi : lo;
-                    *reinterpret_cast<float4*>(to + ((j % 32 / 4 + !odd ^ g8) << 4)) = odd ? lo : hi;
-                }
-                ptx::fence_proxy_async_smem();
-                ptx::tc_fence_before();
-            }
+            cp_async_wait<C::WTILES - 1>();
+            ptx::fence_proxy_async_smem();
+            ptx::tc_fence_before();
             ok = __syncthreads_and(ok);        // B is there, the former rows have been read from tensor memory
             if (!ok) break;
             ptx::tc_fence_after();
             ++issued;
             if (warp == 0) {
-#pragma unroll 1
-                for (int k = 0; 32 * k < rank; ++k) {
-                    mma_tf32_block_warp(tmem, ptx::desc_lo(wtile + k * C::WBLOCK, 16), ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16), dhi, idesc, k > 0);
-                }
+                const uint32_t tile = area_s + C::W_AT + (c - first) % C::WTILES * C::WTILE;
+#pragma unroll
+                for (int k = 0; k < C::BLOCKS; ++k)
+                    mma_f16_block_warp(tmem, ptx::desc_lo(tile + k * C::WBLOCK, 16), ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16), dhi, idesc, k > 0);
                 ptx::mma_commit_warp(bar + 8);
             }
-            load_w(c + 1);
             ok = ptx::mbar_wait_warp(bar + 8, (c - first) & 1, abort_flag);
             ptx::tc_fence_after();
-            // rows 4 g and + 1 in the first, + 2 and + 3 in the second; tokens 8 i + 2 t and + 1; the remainders' part 32 columns on
-            uint32_t ra[HALF / 2], rb[HALF / 2], qa[HALF / 2], qb[HALF / 2];
-            const int nw = HALF * (warp >> 2), row = 128 * c + 32 * (warp & 3) + 4 * g;
+            fetch_b(c + C::WTILES);            // in the place of the tile just used
+            // rows 4 g and + 1 in the first, + 2 and + 3 in the second; tokens 8 i + 2 t and + 1; a part 32 columns behind the other
+            uint32_t ra[T::PARTS][COLS / 2], rb[T::PARTS][COLS / 2];
+            const int row = 128 * c + 32 * (warp & 3) + 4 * g;
             const uint32_t from = tmem + (uint32_t(32 * (warp & 3)) << 16) + nw;
-            ptx::tmem_ld16x256_cols(from, ra);
-            ptx::tmem_ld16x256_cols(from + (16u << 16), rb);
-            ptx::tmem_ld16x256_cols(from + AD_TOK, qa);
-            ptx::tmem_ld16x256_cols(from + (16u << 16) + AD_TOK, qb);
-            ptx::tmem_wait_ld_tied(ra);
-            ptx::tmem_wait_ld_tied(rb);
-            ptx::tmem_wait_ld_tied(qa);
-            ptx::tmem_wait_ld_tied(qb);
+#pragma unroll
+            for (int k = 0; k < T::PARTS; ++k) {
+                ptx::tmem_ld16x256_cols(from + k * AD_TOK, ra[k]);
+                ptx::tmem_ld16x256_cols(from + k * AD_TOK + (16u << 16), rb[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < T::PARTS; ++k) {
+                ptx::tmem_wait_ld_tied(ra[k]);
+                ptx::tmem_wait_ld_tied(rb[k]);
+            }
             ptx::tc_fence_before();
-            auto sum = [](uint32_t x, uint32_t y) { return __uint_as_float(x) + __uint_as_float(y); };
+            auto sum = [&](uint32_t (&r)[T::PARTS][COLS / 2], int i, float by) {
+                float v = __uint_as_float(r[T::PARTS - 1][i]);
+#pragma unroll
+                for (int k = T::PARTS - 2; k >= 0; --k) v += __uint_as_float(r[k][i]);
+                return T::PARTS == 2 ? v * by : v;
+            };
             float* yrow = p.Y + (n0 + nw) * p.ldy + P.row0 + row;
             if (ok && row < P.rows)
 #pragma unroll
-                for (int i = 0; i < HALF / 8; ++i)
+                for (int i = 0; i < COLS / 8; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int n = 8 * i + 2 * t + e;
-                        if (nw + n < live)
-                            add_to4(yrow + n * p.ldy, sum(ra[4 * i + e], qa[4 * i + e]), sum(ra[4 * i + 2 + e], qa[4 * i + 2 + e]), sum(rb[4 * i + e], qb[4 * i + e]),
-                                    sum(rb[4 * i + 2 + e], qb[4 * i + 2 + e]));
+                        const float by = e ? down[i].y : down[i].x;
+                        if (nw + n < live) add_to4(yrow + n * p.ldy, sum(ra, 4 * i + e, by), sum(ra, 4 * i + 2 + e, by), sum(rb, 4 * i + e, by), sum(rb, 4 * i + 2 + e, by));
                     }
         }
+        cp_async_wait<0>();
         ok = __syncthreads_and(ok);
         if (tid == 0 && !ok && wanted) {
             atomicOr(&g_dense_err, ERR_WAIT_FOLD);
@@ -493,7 +495,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             if (issued) ptx::mbar_wait(bar + 8, (issued - 1) & 1, abort_flag);
         }
         __syncthreads();
-        if (warp == 0) ptx::tmem_dealloc(tmem, 2 * AD_TOK);
+        if (warp == 0) ptx::tmem_dealloc(tmem, 128);
     } else {
         if (!ok) {
             if (tid == 0) {
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             if constexpr (T::PARTS == 2)
 #pragma unroll
                 for (int nt = 0; nt < 4; ++nt) {
-                    const float2 u = *reinterpret_cast<const float2*>(hs + AD_TOK * (C::LDH + C::LDH3) + 4 * (8 * nt + 2 * t));
+                    const float2 u = *reinterpret_cast<const float2*>(area + C::UP_AT + 4 * (8 * nt + 2 * t));
 #pragma unroll
                     for (int i = 0; i < 2; ++i) { acc[i][nt][0] *= u.x; acc[i][nt][1] *= u.y; acc[i][nt][2] *= u.x; acc[i][nt][3] *= u.y; }
                 }
@@ -565,8 +567,8 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
 
 namespace {
 // CTAs of a cluster, by the sizes alone (the segments are on the device): as many as fit on the chip at once, two an SM where their shared memory lets
-// them. In a graph, with 1 / 2 / 4 / 8 of them: rank 16, 1 token 14.2 / 8.8 / 6.2 / 5.0 us, 64 segments of 32 tokens 21.6 / 14.1 / 13.4 / 18.2, 4096 tokens
-// 24.4 / 21.4 / 27.7 / -; rank 64, 8 segments of 128 tokens 35.5 / 20.7 / 14.2 / 31, 4096 tokens 35.8 / 31.1 / 37.0 / -.
+// them. In a graph, with 2 / 4 / 8 of them: rank 16, 1 token 8.7 / 6.0 / 4.9 us, 64 segments of 32 tokens 13.3 / 13.0 / 18.2, 4096 tokens
+// 20.5 / 26.4 / -; rank 64, 2 segments of 128 tokens 18.4 / 11.8 / 9.4, 8 of them 19.3 / 13.0 / 29.6, 4096 tokens 28.7 / 32.9 / 86.
 template <int RT> int adapter_parts(long long ntokens, long long nseg, int npools, int sms) {
     const long long tiles = std::max(std::min(nseg, ntokens), (ntokens + llattn::AD_TOK - 1) / llattn::AD_TOK) * npools;
     int parts = llattn::AdapterTile<RT>::MOST;
