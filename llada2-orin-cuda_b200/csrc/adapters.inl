@@ -566,40 +566,54 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
 }  // namespace llattn
 
 namespace {
-// CTAs of a cluster, by the sizes alone (the segments are on the device): as many as fit on the chip at once, two an SM where their shared memory lets
-// them. In a graph, with 2 / 4 / 8 of them: rank 16, 1 token 8.7 / 6.0 / 4.9 us, 64 segments of 32 tokens 13.3 / 13.0 / 18.2, 4096 tokens
-// 20.5 / 26.4 / -; rank 64, 2 segments of 128 tokens 18.4 / 11.8 / 9.4, 8 of them 19.3 / 13.0 / 29.6, 4096 tokens 28.7 / 32.9 / 86.
-template <int RT> int adapter_parts(long long ntokens, long long nseg, int npools, int sms) {
-    const long long tiles = std::max(std::min(nseg, ntokens), (ntokens + llattn::AD_TOK - 1) / llattn::AD_TOK) * npools;
-    int parts = llattn::AdapterTile<RT>::MOST;
-    while (parts > 1 && parts * tiles > (llattn::AdapterTile<RT>::bytes(parts) <= 113 * 1024 ? 2 : 1) * sms) parts /= 2;
-    return parts;
-}
-
+// CTAs of a cluster, by the sizes alone (the segments are on the device): as many as are on the chip at once, two an SM where their shared memory lets
+// them. How many clusters of 2, 4 and 8 there are with one CTA an SM is asked of the runtime (74, 33 and 15: groups of SMs are not multiples of eight).
+// In a graph, with 2 / 4 / 8 CTAs: rank 16, 1 token 8.7 / 6.0 / 4.9 us, 32 tiles 11.0 / 8.7 / 8.9, 64 (segments of 32 tokens) 13.2 / 13.0 / 18.2, 128 20.5 / 26.4 /
+// -; rank 64, 8 tiles 18.3 / 11.7 / 9.4, 18 11.5 / 8.5 / 14.6, 32 19.2 / 13.0 / 29.6, 128 28.7 / 32.9 / 86.
 template <typename T, int RT>
-int launch_adapters(llattn::AdapterParams& p, int npools, int sms, cudaStream_t stream) {
+int launch_adapters(llattn::AdapterParams& p, int npools, cudaStream_t stream) {
     using namespace llattn;
-    static std::atomic<bool> ready[64];
+    using C = AdapterTile<RT>;
+    constexpr int ONE_AN_SM = 200 * 1024, TWO_AN_SM = 113 * 1024;
+    static std::mutex mu;
+    static int clusters[64][3];                // by device; the first one 0: not asked yet
     auto* kernel = adapters_kernel<T, RT>;
-    constexpr int most = AdapterTile<RT>::bytes(AdapterTile<RT>::MOST);
-    int dev = 0;
+    int dev = 0, fit[3];
     CU(cudaGetDevice(&dev));
-    if (most > 48 * 1024 && (dev >= 64 || !ready[dev])) {
-        CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-        if (dev < 64) ready[dev] = true;
+    if (dev >= 64) return fail(LLATTN_EINVAL, "adapters_w4a8: device index %d not supported", dev);
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!clusters[dev][0]) {
+            CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(C::bytes(C::MOST), ONE_AN_SM)));
+            for (int i = 2; i >= 0; --i) {
+                cudaLaunchConfig_t cfg{};
+                cudaLaunchAttribute attr{};
+                attr.id = cudaLaunchAttributeClusterDimension;
+                attr.val.clusterDim.x = 2 << i; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+                cfg.gridDim = dim3(2 << i); cfg.blockDim = dim3(AD_THREADS); cfg.dynamicSmemBytes = ONE_AN_SM;
+                cfg.attrs = &attr; cfg.numAttrs = 1;
+                int n = 0;
+                CU(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+                clusters[dev][i] = i ? n : std::max(n, 1);
+            }
+        }
+        for (int i = 0; i < 3; ++i) fit[i] = 2 << i > C::MOST ? 0 : clusters[dev][i] * (C::bytes(2 << i) <= TWO_AN_SM ? 2 : 1);
     }
-    p.parts = adapter_parts<RT>(p.ntokens, p.nseg, npools, sms);
+    const long long work = std::max<long long>(std::min(p.nseg, p.ntokens), (p.ntokens + AD_TOK - 1) / AD_TOK) * npools;       // tiles, in the mean
+    p.parts = 1;
+    for (int i = 0; i < 3; ++i)
+        if (work <= fit[i]) p.parts = 2 << i;
     // no more tiles than this, however the segments cut the tokens: each has at most one that is not full
     const long long tiles = std::min<long long>(p.ntokens, (p.ntokens + (AD_TOK - 1ll) * p.nseg) / AD_TOK);
-    CU(launch_dependent_cluster(kernel, dim3(unsigned(tiles * p.parts), npools), AD_THREADS, AdapterTile<RT>::bytes(p.parts), p.parts, stream, p));
+    CU(launch_dependent_cluster(kernel, dim3(unsigned(tiles * p.parts), npools), AD_THREADS, C::bytes(p.parts), p.parts, stream, p));
     return LLATTN_OK;
 }
 template <typename T>
-int launch_adapters_rank(llattn::AdapterParams& p, int npools, int rank, int sms, cudaStream_t stream) {
-    if (rank <= 16) return launch_adapters<T, 1>(p, npools, sms, stream);
-    if (rank <= 32) return launch_adapters<T, 2>(p, npools, sms, stream);
-    if (rank <= 64) return launch_adapters<T, 4>(p, npools, sms, stream);
-    return launch_adapters<T, 8>(p, npools, sms, stream);
+int launch_adapters_rank(llattn::AdapterParams& p, int npools, int rank, cudaStream_t stream) {
+    if (rank <= 16) return launch_adapters<T, 1>(p, npools, stream);
+    if (rank <= 32) return launch_adapters<T, 2>(p, npools, stream);
+    if (rank <= 64) return launch_adapters<T, 4>(p, npools, stream);
+    return launch_adapters<T, 8>(p, npools, stream);
 }
 }  // namespace
 
@@ -643,9 +657,6 @@ extern "C" int llattn_adapters_w4a8(const llattn_adapter_pool* pools, int npools
     if (ntokens == 0 || nseg == 0) return LLATTN_OK;
     p.q = q; p.s = s; p.Y = Y; p.first = seg_first; p.adapter = seg_adapter;
     p.ldy = ldy; p.ntokens = ntokens; p.K = K; p.nseg = nseg;
-    int dev = 0, sms = 0;
-    CU(cudaGetDevice(&dev));
-    CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    return pools[0].type == LLATTN_F16 ? launch_adapters_rank<AdapterF16>(p, npools, rank, sms, as_stream(stream))
-                                       : launch_adapters_rank<AdapterBF16>(p, npools, rank, sms, as_stream(stream));
+    return pools[0].type == LLATTN_F16 ? launch_adapters_rank<AdapterF16>(p, npools, rank, as_stream(stream))
+                                       : launch_adapters_rank<AdapterBF16>(p, npools, rank, as_stream(stream));
 }
