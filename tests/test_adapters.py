@@ -248,6 +248,42 @@ def test_nothing_to_do(api):
     api.qkv_prepare_commit_axes(z(0, 3072), z(2, 0, dtype=i32), axes, z(128), z(128), 1e-6, freq, *out, z(4, 1, 4736, dtype=torch.uint8), max_blocks=1)
 
 
+@pytest.mark.gpu
+def test_adapters_on_two_streams_at_once(api, orc, pkg):
+    """Calls of every kernel that overlap on the device, a tcgen05 projection between them, give the bits of calls one at a time."""
+    T, K, n, parts = 700, 512, 3, [(0, 512)]
+    strips = torch.from_numpy(pkg.workload.dense_weights(512, K, 1)[0]).cuda()
+    jobs = []
+    for k, (rank, dtype) in enumerate([(16, F16), (64, BF16), (128, F16), (32, BF16), (64, F16), (8, BF16)]):
+        q, s, Y, ab = _case(T, K, rank, n, parts, dtype, k)
+        first, adapter = _random_segments(T, 9, n, k)
+        dev = lambda a, t=None: torch.from_numpy(np.ascontiguousarray(a)).cuda()
+        qsum = dev(q.reshape(T, K // 128, 128).sum(2, dtype=np.int32))
+        pools = api.adapter_pools([api.AdapterPool(*[x.cuda() for x in ab[0]])])
+        jobs.append((pools, dev(q), dev(s), qsum, dev(Y[:, :512]), dev(np.asarray(first, np.int32)), dev(np.asarray(adapter, np.int32))))
+    torch.cuda.synchronize()
+
+    def run(streams):
+        outs = []
+        for i, (pools, q, s, qsum, Y, first, adapter) in enumerate(jobs):
+            with torch.cuda.stream(streams[i % len(streams)]):
+                y = Y.clone()
+                for _ in range(3):
+                    api.adapters_w4a8(pools, q, s, y, first, adapter)
+                    api.dense_w4a8(strips, q, s, qsum, y)
+                outs.append(y)
+            if len(streams) == 1:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+
+    want = run([torch.cuda.current_stream()])
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(want, run(streams)))
+    assert api.dense_status() == 0 and all(bool(torch.isfinite(a).all()) for a in want)
+
+
 def _args(api, **changed):
     """A call of the C entry point with addresses that no check refuses, but for what is changed. Nothing is launched: a call that passes has no tokens."""
     pool = dict(A=0x100000, B=0x200000, scale=0x300000, ranks=0x310000, n=4, rank=16, rows=64, row0=0, type=api.F16)
