@@ -213,23 +213,31 @@ int llattn_kv_commit_paged(const void* Kf, const void* Vf, void* pool, const int
 
 // ------------------------------------------------------------------------------------------------------ producer
 
+}  // extern "C"
+
 namespace {
+template <bool AXES>
+int launch_prepare(const llattn::PrepArgs& a, cudaStream_t stream) {
+    using namespace llattn;
+    const int blocks = (a.T + BLK - 1) / BLK;
+    int dev = 0, sms = 0;
+    if (a.records) { CU(cudaGetDevice(&dev)); CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)); }
+    if (!a.records) CU(launch_dependent(qkv_prepare_kernel<false, PREP_THREADS, AXES>, dim3(blocks, 6 * prep_parts(PREP_THREADS)), PREP_THREADS, stream, a));
+    else if (9 * (long long)blocks <= 4 * sms)
+        CU(launch_dependent(qkv_prepare_kernel<true, PREP_FEW_THREADS, AXES>, dim3(blocks, NKV + 4 * prep_parts(PREP_FEW_THREADS)), PREP_FEW_THREADS, stream, a));
+    else CU(launch_dependent(qkv_prepare_kernel<true, PREP_THREADS, AXES>, dim3(blocks, NKV + 4 * prep_parts(PREP_THREADS)), PREP_THREADS, stream, a));
+    return LLATTN_OK;
+}
+// axis_of 0: one axis (with several, frequencies that are all on the first are the same thing)
 int launch_prepare(const float* qkv, const int32_t* pos, const float* gq, const float* gk, float eps, const float* inv_freq,
                    void* q, void* k, void* v, int T, uint64_t axis_of, void* records, const int32_t* pages, int max_blocks, int blk, void* stream) {
-    llattn::PrepArgs a{qkv, pos, gq, gk, inv_freq, eps, static_cast<half*>(q), static_cast<half*>(k), static_cast<half*>(v), T, axis_of,
-                       static_cast<uint8_t*>(records), pages, max_blocks, blk};
-    const int blocks = (T + llattn::BLK - 1) / llattn::BLK;
-    using namespace llattn;
-    int dev = 0, sms = 0;
-    if (records) { CU(cudaGetDevice(&dev)); CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)); }
-    if (!records) CU(launch_dependent(qkv_prepare_kernel<false, PREP_THREADS>, dim3(blocks, 6 * prep_parts(PREP_THREADS)), PREP_THREADS, as_stream(stream), a));
-    else if (9 * (long long)blocks <= 4 * sms)
-        CU(launch_dependent(qkv_prepare_kernel<true, PREP_FEW_THREADS>, dim3(blocks, NKV + 4 * prep_parts(PREP_FEW_THREADS)), PREP_FEW_THREADS, as_stream(stream), a));
-    else CU(launch_dependent(qkv_prepare_kernel<true, PREP_THREADS>, dim3(blocks, NKV + 4 * prep_parts(PREP_THREADS)), PREP_THREADS, as_stream(stream), a));
-    return LLATTN_OK;
+    const llattn::PrepArgs a{qkv, pos, gq, gk, inv_freq, eps, static_cast<half*>(q), static_cast<half*>(k), static_cast<half*>(v), T, axis_of,
+                             static_cast<uint8_t*>(records), pages, max_blocks, blk};
+    return axis_of ? launch_prepare<true>(a, as_stream(stream)) : launch_prepare<false>(a, as_stream(stream));
 }
 }  // namespace
 
+extern "C" {
 namespace {
 int prepare_only(const char* who, const float* qkv, const int32_t* pos, const float* gq, const float* gk, float eps, const float* inv_freq,
                  void* q, void* k, void* v, int T, uint64_t axis_of, void* stream) {
