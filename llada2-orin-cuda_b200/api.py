@@ -153,23 +153,23 @@ _torch_of = None
 
 
 def _torch():
-    """(torch, LLATTN_F32 / F16 / BF16 by dtype, the current device's index)"""
+    """(float32, float16, int8, int32, LLATTN_F32 / F16 / BF16 by dtype, current device's index, current stream's handle on a device)"""
     global _torch_of
-    if _torch_of is None:
-        import torch
-        types, device = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}, getattr(torch._C, "_cuda_getDevice", None)
-        if device is None or not torch.cuda.is_initialized():
-            return torch, types, torch.cuda.current_device()
-        _torch_of = torch, types, device
-    torch, types, device = _torch_of
-    return torch, types, device()
+    if _torch_of is not None:
+        return _torch_of
+    import torch
+    device, handle = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    of = lambda d, h: (torch.float32, torch.float16, torch.int8, torch.int32, types, d, h)
+    if device is None or handle is None or not torch.cuda.is_initialized():      # the long way, and before CUDA is up
+        return of(torch.cuda.current_device, lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+    _torch_of = of(device, handle)
+    return _torch_of
 
 
-def _flat(t, dtype, n: int, dev: int, what: str) -> int:
-    """Data pointer of a contiguous tensor of n values on device `dev`, the current one: that is where the launch goes, whatever the pointers."""
-    if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError(f"{what}: {n} contiguous values of {dtype} on cuda:{dev}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
-    return t.data_ptr()
+def _refuse(who: str, wanted: str, **tensors):
+    raise ValueError(f"{who}: {wanted}, all contiguous on the current device; got " +
+                     ", ".join(f"{k} {tuple(t.shape)} of {t.dtype} on {t.device}" for k, t in tensors.items() if t is not None))
 
 
 def _rows(t, dtype, T: int, K: int, dev: int, what: str):
@@ -349,39 +349,46 @@ def rope_axes(sections, interleaved: bool = False) -> bytes:
     return bytes(out)
 
 
-def _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v):
-    torch, _, dev = _torch()
-    T = qkv.shape[0]
-    if pos.dim() != 2 or pos.shape[1] != T or len(axis_of) != 32:
-        raise ValueError("pos is int32 [axes][T], axis_of one axis for each of the 32 frequencies")
-    f32, f16, naxes = torch.float32, torch.float16, pos.shape[0]
-    return T, (_flat(qkv, f32, T * (NQH + 2 * NKV) * D, dev, "qkv"), _flat(pos, torch.int32, naxes * T, dev, "pos"), naxes, bytes(axis_of),
-               _flat(gq, f32, D, dev, "gq"), _flat(gk, f32, D, dev, "gk"), eps, _flat(inv_freq_t, f32, 32, dev, "inv_freq"),
-               _flat(q, f16, T * NQH * D, dev, "q"), _flat(k, f16, T * NKV * D, dev, "k"), _flat(v, f16, T * NKV * D, dev, "v"))
+# The checks of these calls are written out: a helper called for each tensor costs 0.1 us a tensor, of a call of 7 us on the host. The device matters: the
+# launch goes to the current one, whatever the pointers.
+def _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream):
+    f32, f16, _, i32, _, device, handle = _torch()
+    dev, T = device(), qkv.shape[0]
+    n = T * NKV * D
+    if (qkv.dtype is not f32 or qkv.numel() != 6 * n or qkv.get_device() != dev or not qkv.is_contiguous() or
+            pos.dtype is not i32 or pos.dim() != 2 or pos.shape[1] != T or pos.get_device() != dev or not pos.is_contiguous() or
+            gq.dtype is not f32 or gq.numel() != D or gq.get_device() != dev or not gq.is_contiguous() or
+            gk.dtype is not f32 or gk.numel() != D or gk.get_device() != dev or not gk.is_contiguous() or
+            inv_freq_t.dtype is not f32 or inv_freq_t.numel() != 32 or inv_freq_t.get_device() != dev or not inv_freq_t.is_contiguous() or
+            q.dtype is not f16 or q.numel() != 4 * n or q.get_device() != dev or not q.is_contiguous() or
+            k.dtype is not f16 or k.numel() != n or k.get_device() != dev or not k.is_contiguous() or
+            v.dtype is not f16 or v.numel() != n or v.get_device() != dev or not v.is_contiguous() or len(axis_of) != 32):
+        _refuse("axes", "qkv fp32 [T][3072], pos int32 [axes][T], 32 axes, gq and gk fp32 [128], inv_freq fp32 [32], q fp16 [T][16][128], k and v fp16 [T][4][128]",
+                qkv=qkv, pos=pos, gq=gq, gk=gk, inv_freq=inv_freq_t, q=q, k=k, v=v)
+    return T, dev, (handle(dev) if stream is None else _stream(stream)), (
+        qkv.data_ptr(), pos.data_ptr(), pos.shape[0], bytes(axis_of), gq.data_ptr(), gk.data_ptr(), eps, inv_freq_t.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr())
 
 
 def qk_norm_rope_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream=None) -> None:
     """qk_norm_rope with several position axes: pos int32 [axes][T], axis_of the axis of each of the 32 frequencies (host; see rope_axes)."""
-    T, args = _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v)
-    if T == 0:                               # (an empty tensor has no address)
-        return
-    _check(lib().llattn_qk_norm_rope_axes(*args, T, _stream(stream)))
+    T, _, st, args = _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream)
+    if T:                                    # (an empty tensor has no address)
+        _check(lib().llattn_qk_norm_rope_axes(*args, T, st))
 
 
 def qkv_prepare_commit_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, cache, max_blocks: int = 0, blk: int = 0, pages=None,
                             stream=None) -> None:
     """qkv_prepare_commit with several position axes, see qk_norm_rope_axes."""
-    T, args = _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v)
-    torch, _, dev = _torch()
+    T, dev, st, args = _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream)
     nb = T // BLK
     if T % BLK:
         raise ValueError("a prefill pass commits whole 32-token blocks")
     if pages is None and cache.numel() < NKV * max_blocks * KV_BLOCK_BYTES:
         raise ValueError("the cache holds fewer than max_blocks blocks")
-    if T == 0:
-        return
-    _check(lib().llattn_qkv_prepare_commit_axes(*args, nb, _flat(cache, torch.uint8, cache.numel(), dev, "cache"),
-                                                None if pages is None else _flat(pages, torch.int32, nb * NKV, dev, "pages"), max_blocks, blk, _stream(stream)))
+    if cache.get_device() != dev or cache.element_size() != 1 or (pages is not None and (pages.get_device() != dev or pages.numel() != nb * NKV or pages.element_size() != 4)):
+        _refuse("axes", "cache uint8, pages int32 [nb][4]", cache=cache, pages=pages)
+    if T:
+        _check(lib().llattn_qkv_prepare_commit_axes(*args, nb, _ptr(cache), _ptr(pages), max_blocks, blk, st))
 
 
 # ------------------------------------------------------------------ norm, adapters
@@ -390,24 +397,32 @@ def add_norm_q8(x, gain, eps, q=None, s=None, qsum=None, delta=None, y=None, str
     """Residual addition, RMS norm and int8 activations in one pass (llattn_add_norm_q8). x fp32 [T][K] takes delta (fp32, fp16 or bf16 [T][K];
     None: nothing is added and x is only read); q int8 [T][K] in fragment order, s fp32 and qsum int32 [T][K/128] are what dense_w4a8 and
     adapters_w4a8 read; y fp16 or bf16 [T][K] the normalised values. The rows of x and delta may be further apart than K."""
-    torch, types, dev = _torch()
+    f32, _, i8, i32, types, device, handle = _torch()
+    dev = device()
     T, K = x.shape
-    xp, ldx = _rows(x, torch.float32, T, K, dev, "x")
+    n, m = T * K, T * (K // 128)
+    xp, ldx = _rows(x, f32, T, K, dev, "x")
     dp, ldd, dtype, qp, sp, sump, yp, ytype = None, 0, 0, None, None, None, None, 0
     if delta is not None:
         dp, ldd = _rows(delta, None, T, K, dev, "delta")
         dtype = types.get(delta.dtype, -1)
-    if q is not None:
-        if s is None or qsum is None:
-            raise ValueError("q, s and qsum go together")
-        qp, sp, sump = _flat(q, torch.int8, T * K, dev, "q"), _flat(s, torch.float32, T * (K // 128), dev, "s"), _flat(qsum, torch.int32, T * (K // 128), dev, "qsum")
-    elif s is not None or qsum is not None:
+    if q is not None and s is not None and qsum is not None:
+        if (q.dtype is not i8 or q.numel() != n or q.get_device() != dev or not q.is_contiguous() or
+                s.dtype is not f32 or s.numel() != m or s.get_device() != dev or not s.is_contiguous() or
+                qsum.dtype is not i32 or qsum.numel() != m or qsum.get_device() != dev or not qsum.is_contiguous()):
+            _refuse("add_norm_q8", "q int8 [T][K], s fp32 and qsum int32 [T][K / 128]", x=x, q=q, s=s, qsum=qsum)
+        qp, sp, sump = q.data_ptr(), s.data_ptr(), qsum.data_ptr()
+    elif q is not None or s is not None or qsum is not None:
         raise ValueError("q, s and qsum go together")
     if y is not None:
-        yp, ytype = _flat(y, y.dtype, T * K, dev, "y"), types.get(y.dtype, -1)
-    if T == 0:                               # (an empty tensor has no address)
-        return
-    _check(lib().llattn_add_norm_q8(xp, ldx, dp, dtype, ldd, _flat(gain, torch.float32, K, dev, "gain"), eps, qp, sp, sump, yp, ytype, T, K, _stream(stream)))
+        if y.numel() != n or y.get_device() != dev or not y.is_contiguous():
+            _refuse("add_norm_q8", "y [T][K]", x=x, y=y)
+        yp, ytype = y.data_ptr(), types.get(y.dtype, -1)
+    if gain.dtype is not f32 or gain.numel() != K or gain.get_device() != dev or not gain.is_contiguous():
+        _refuse("add_norm_q8", "gain fp32 [K]", x=x, gain=gain)
+    if T:                                    # (an empty tensor has no address)
+        _check(lib().llattn_add_norm_q8(xp, ldx, dp, dtype, ldd, gain.data_ptr(), eps, qp, sp, sump, yp, ytype, T, K,
+                                        handle(dev) if stream is None else _stream(stream)))
 
 
 @dataclass
@@ -429,7 +444,7 @@ class AdapterPool:
         if (self.scale is not None and (self.scale.numel() != n or self.scale.dtype != torch.float32)) or \
            (self.ranks is not None and (self.ranks.numel() != n or self.ranks.dtype != torch.int32)):
             raise ValueError("scale is fp32 [n], ranks int32 [n]")
-        return _AdapterPool(_ptr(A), _ptr(B), _ptr(self.scale), _ptr(self.ranks), n, A.shape[1], B.shape[1], self.row0, _torch()[1].get(A.dtype, -1))
+        return _AdapterPool(_ptr(A), _ptr(B), _ptr(self.scale), _ptr(self.ranks), n, A.shape[1], B.shape[1], self.row0, _torch()[4].get(A.dtype, -1))
 
 
 class AdapterPools:
@@ -455,16 +470,22 @@ def adapters_w4a8(pools: AdapterPools, q, s, Y, seg_first, seg_adapter, stream=N
     """Adds the adapters of many requests to a projection's output Y (fp32 [ntokens][>= row0 + rows], rows contiguous), from the activations
     (q int8 [ntokens][K] in fragment order, s fp32 [ntokens][K/128]) that dense_w4a8 reads (llattn_adapters_w4a8). Segment i is the tokens
     seg_first[i] .. seg_first[i + 1] - 1 and has adapter seg_adapter[i] (-1: none); both are int32 device tensors."""
-    torch, _, dev = _torch()
+    f32, _, i8, i32, _, device, handle = _torch()
+    dev = device()
     T, width = Y.shape
-    K, nseg, f32, i32 = pools.K, seg_adapter.numel(), torch.float32, torch.int32
+    K, nseg = pools.K, seg_adapter.numel()
     if pools._rows > width or pools.device != dev:
         raise ValueError(f"the pools' rows reach to {pools._rows} of {width}, on cuda:{pools.device}; the current device is cuda:{dev}")
+    if (q.dtype is not i8 or q.numel() != T * K or q.get_device() != dev or not q.is_contiguous() or
+            s.dtype is not f32 or s.numel() != T * (K // 128) or s.get_device() != dev or not s.is_contiguous() or
+            seg_first.dtype is not i32 or seg_first.numel() != nseg + 1 or seg_first.get_device() != dev or not seg_first.is_contiguous() or
+            seg_adapter.dtype is not i32 or seg_adapter.get_device() != dev or not seg_adapter.is_contiguous()):
+        _refuse("adapters_w4a8", f"q int8 [T][{K}], s fp32 [T][{K // 128}], seg_first int32 [segments + 1], seg_adapter int32 [segments]", Y=Y, q=q, s=s, seg_first=seg_first,
+                seg_adapter=seg_adapter)
     yp, ldy = _rows(Y, f32, T, width, dev, "Y")
-    if T == 0 or nseg == 0:                  # (an empty tensor has no address)
-        return
-    _check(lib().llattn_adapters_w4a8(pools._c, len(pools._c), _flat(q, torch.int8, T * K, dev, "q"), _flat(s, f32, T * (K // 128), dev, "s"), yp, ldy, T, K,
-                                      _flat(seg_first, i32, nseg + 1, dev, "seg_first"), _flat(seg_adapter, i32, nseg, dev, "seg_adapter"), nseg, _stream(stream)))
+    if T and nseg:                           # (an empty tensor has no address)
+        _check(lib().llattn_adapters_w4a8(pools._c, len(pools._c), q.data_ptr(), s.data_ptr(), yp, ldy, T, K, seg_first.data_ptr(), seg_adapter.data_ptr(), nseg,
+                                          handle(dev) if stream is None else _stream(stream)))
 
 
 # ------------------------------------------------------------------ the reference operator pair
