@@ -23,7 +23,7 @@
 //
 // What bounds it: one token 4.9 us, a chain of launch, segment, operands, the cluster's exchange (1.2 us) and B. A full batch (64 segments of 32 tokens,
 // adapters of rank 16) 13.0 us = 3.5 TB/s cold and 10.0 warm, of which 9.1 without the additions to Y: reading, computing and adding
-// overlap only across CTAs, and the chip holds all of them at once. 4096 tokens of rank 64 28.7 us, issue slots and shared memory of the first product
+// overlap only across CTAs, and the chip holds all of them at once. 4096 tokens of rank 64 28.5 us, issue slots and shared memory of the first product
 // (45 %), the second product's tiles (the rest); with tf32 pairs on mma.sync 45, with one CTA a tile and every operand from memory 205.
 #pragma once
 
@@ -121,13 +121,15 @@ template <int RT> struct AdapterTile {
     // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
     static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : RT > 1 ? 3 : 5;
     // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], and H in parts of 16 bits. For few ranks the first two parts [TOK]
-    // rows LDH bytes apart, and the third; else the tensor cores' tiles, 64 ranks a block, and behind them tiles of 128 rows of B. A power of two for each
+    // rows LDH bytes apart, and the third; else the tensor cores' tiles, 64 ranks a block, and behind them tiles of 128 rows of B, the last one where the sums were. A power of two for each
     // token. In front of all a slot [TOK][R] for the sums of each other CTA of the cluster.
     static constexpr bool WIDE = RT >= 4;
     static constexpr int LDP = R + 4, LDH = 4 * R + (RT == 2 ? 64 : 0), LDH3 = LDH / 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
-    static constexpr int BLOCKS = (R + 63) / 64, HBLOCK = 3 * TOK * 128, WBLOCK = 128 * 128, WTILE = BLOCKS * WBLOCK, WTILES = RT > 4 ? 1 : 2;
+    static constexpr int BLOCKS = (R + 63) / 64, HBLOCK = 3 * TOK * 128, WBLOCK = 128 * 128, WTILE = BLOCKS * WBLOCK, WTILES = RT > 4 ? 2 : 3;
     static constexpr int H_AT = WIDE ? (SUMS + 1023) / 1024 * 1024 : SUMS, W_AT = H_AT + BLOCKS * HBLOCK;
-    static constexpr int UP_AT = WIDE ? W_AT + WTILES * WTILE : H_AT + TOK * (LDH + LDH3), AREA = UP_AT + TOK * 4;
+    static constexpr int UP_AT = WIDE ? W_AT + (WTILES - 1) * WTILE : H_AT + TOK * (LDH + LDH3), AREA = UP_AT + TOK * 4;
+    static_assert(!WIDE || WTILE <= H_AT, "the last tile takes the place of the sums");
+    static __device__ __forceinline__ int tile_at(int i) { return i % WTILES == WTILES - 1 ? 0 : W_AT + i % WTILES * WTILE; }
     static constexpr int HEAD = WIDE ? 1024 : 64;
     static constexpr int bytes(int ctas) { return HEAD + (ctas - 1) * SLOT + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
     static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : 4;        // CTAs of a cluster
@@ -220,13 +222,14 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         if (tid == 0) atomicOr(&g_dense_err, ERR_SMEM_ALIGN);
         return;
     }
-    // ---- barriers: one counts the sums of the cluster's CTAs in (they may use it once all are here), one the tensor cores' products
+    // ---- barriers: one counts the sums of the cluster's CTAs in (they may use it once all are here), two the tensor cores' products
     const uint32_t bar = ptx::smem_u32(ad_smem), slots_s = ptx::smem_u32(ad_smem + C::HEAD);
-    volatile int* abort_flag = reinterpret_cast<int*>(ad_smem + 16);
+    volatile int* abort_flag = reinterpret_cast<int*>(ad_smem + 24);
     if (tid == 0) {
         *abort_flag = 0;
         ptx::mbar_init(bar, 1);
         ptx::mbar_init(bar + 8, 1);
+        ptx::mbar_init(bar + 16, 1);
         ptx::fence_mbar_init();
         if (parts > 1) ptx::mbar_arrive_expect_tx(bar, (parts - 1) * C::SLOT);
     }
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
     };
     for (int i = 0; i < C::STAGES - 1; ++i) fetch(i);
     if constexpr (C::WIDE)
-        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 20), 128); ptx::tmem_relinquish(); }
+        if (warp == 0) { ptx::tmem_alloc(ptx::smem_u32(ad_smem + 28), 256); ptx::tmem_relinquish(); }
     const int rank_there = P.ranks ? __ldg(P.ranks + a) : P.rank;  // looked at when the sums are there: a wait for it here would hold up what follows
     const float scale = P.scale ? __ldg(P.scale + a) : 1.f;
     // ---- this CTA's rows of B are wanted when H is done: into L2, and a small rank's first ones into registers
@@ -341,13 +344,13 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             for (int m = 0; m < 128 * C::R / 8; m += AD_THREADS) {
                 const int r = (m + tid) / (C::R / 8), j = (m + tid) % (C::R / 8) * 8, row = 128 * c + r, at = r / 32 * 32 + r / 4 % 8 + r % 4 * 8;
                 const int bytes = row < P.rows ? min(max(rank - j, 0), 8) * 2 : 0;
-                cp_async16_some(area_s + C::W_AT + (c - first) % C::WTILES * C::WTILE + j / 64 * C::WBLOCK + at * 128 + ((j % 64 / 8 ^ (at & 7)) << 4),
+                cp_async16_some(area_s + C::tile_at(c - first) + j / 64 * C::WBLOCK + at * 128 + ((j % 64 / 8 ^ (at & 7)) << 4),
                                 bytes ? B + size_t(row) * P.rank + j : B, bytes);
             }
         cp_async_commit();
     };
     if constexpr (C::WIDE)
-        for (int c = first; c < first + C::WTILES; ++c) fetch_b(c);
+        for (int c = first; c < first + C::WTILES - 1; ++c) fetch_b(c);
     float* sums = reinterpret_cast<float*>(area);
 #pragma unroll
     for (int r = 0; r < C::RW; ++r)
@@ -424,7 +427,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
     if constexpr (C::WIDE) {
         // ---- Y, 128 rows at a time on tcgen05: a tile of B times all parts of H beside one another into tensor memory
         ptx::tc_fence_after();
-        const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 20);
+        const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 28);
         const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = ptx::idesc_f16(128, T::PARTS * AD_TOK, false, false) | T::IDESC;
         constexpr int COLS = AD_TOK / 2;       // of a warp: a quarter of the rows, half of the tokens
         const bool wanted = rank != 0;
@@ -433,30 +436,43 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
 #pragma unroll
         for (int i = 0; i < COLS / 8; ++i) down[i] = T::PARTS == 2 ? *reinterpret_cast<const float2*>(area + C::UP_AT + 4 * (nw + 8 * i + 2 * t)) : make_float2(1.f, 1.f);
         int issued = 0;
-        ok = ok && wanted;
+        auto multiply = [&](int c) {           // by warp 0
+            const uint32_t tile = area_s + C::tile_at(c - first), acc = tmem + ((c - first) & 1) * 128;
+#pragma unroll
+            for (int k = 0; k < C::BLOCKS; ++k)
+                mma_f16_block_warp(acc, ptx::desc_lo(tile + k * C::WBLOCK, 16), ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16), dhi, idesc, k > 0);
+            ptx::mma_commit_warp(bar + 8 + 8 * ((c - first) & 1));
+        };
+        fetch_b(first + C::WTILES - 1);        // the sums have been passed on
+        cp_async_wait<C::WTILES - 1>();
+        ptx::fence_proxy_async_smem();
+        ok = __syncthreads_and(ok && wanted && first < end);
+        if (ok) {
+            if (warp == 0) multiply(first);
+            issued = 1;
+        }
+        // the products of the next rows run while these rows' are on their way to Y: two accumulators (8 segments of 128 tokens of rank 64 13.0 -> 12.2 us)
 #pragma unroll 1
-        for (int c = first; c < end; ++c) {
-            cp_async_wait<C::WTILES - 1>();
-            ptx::fence_proxy_async_smem();
+        for (int c = first; c < end && issued; ++c) {
+            if (c + 1 < end) {
+                cp_async_wait<C::WTILES - 2>();
+                ptx::fence_proxy_async_smem();
+            }
             ptx::tc_fence_before();
             ok = __syncthreads_and(ok);        // B is there, the former rows have been read from tensor memory
             if (!ok) break;
             ptx::tc_fence_after();
-            ++issued;
-            if (warp == 0) {
-                const uint32_t tile = area_s + C::W_AT + (c - first) % C::WTILES * C::WTILE;
-#pragma unroll
-                for (int k = 0; k < C::BLOCKS; ++k)
-                    mma_f16_block_warp(tmem, ptx::desc_lo(tile + k * C::WBLOCK, 16), ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16), dhi, idesc, k > 0);
-                ptx::mma_commit_warp(bar + 8);
+            if (c + 1 < end) {
+                if (warp == 0) multiply(c + 1);
+                ++issued;
             }
-            ok = ptx::mbar_wait_warp(bar + 8, (c - first) & 1, abort_flag);
+            ok = ptx::mbar_wait_warp(bar + 8 + 8 * ((c - first) & 1), ((c - first) >> 1) & 1, abort_flag);
             ptx::tc_fence_after();
             fetch_b(c + C::WTILES);            // in the place of the tile just used
             // rows 4 g and + 1 in the first, + 2 and + 3 in the second; tokens 8 i + 2 t and + 1; a part 32 columns behind the other
             uint32_t ra[T::PARTS][COLS / 2], rb[T::PARTS][COLS / 2];
             const int row = 128 * c + 32 * (warp & 3) + 4 * g;
-            const uint32_t from = tmem + (uint32_t(32 * (warp & 3)) << 16) + nw;
+            const uint32_t from = tmem + ((c - first) & 1) * 128 + (uint32_t(32 * (warp & 3)) << 16) + nw;
 #pragma unroll
             for (int k = 0; k < T::PARTS; ++k) {
                 ptx::tmem_ld16x256_cols(from + k * AD_TOK, ra[k]);
@@ -487,15 +503,17 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         }
         cp_async_wait<0>();
         ok = __syncthreads_and(ok);
-        if (tid == 0 && !ok && wanted) {
+        if (tid == 0 && !ok && wanted && first < end) {
             atomicOr(&g_dense_err, ERR_WAIT_FOLD);
             *abort_flag = 0;
             if (parts > 1) ptx::mbar_wait(bar, 0, abort_flag);                 // stores and products that are still on their way
-            *abort_flag = 0;
-            if (issued) ptx::mbar_wait(bar + 8, (issued - 1) & 1, abort_flag);
+            for (int k = max(0, issued - 2); k < issued; ++k) {
+                *abort_flag = 0;
+                ptx::mbar_wait(bar + 8 + 8 * (k & 1), (k >> 1) & 1, abort_flag);
+            }
         }
         __syncthreads();
-        if (warp == 0) ptx::tmem_dealloc(tmem, 128);
+        if (warp == 0) ptx::tmem_dealloc(tmem, 256);
     } else {
         if (!ok) {
             if (tid == 0) {
@@ -569,7 +587,7 @@ namespace {
 // CTAs of a cluster, by the sizes alone (the segments are on the device): as many as are on the chip at once, two an SM where their shared memory lets
 // them. How many clusters of 2, 4 and 8 there are with one CTA an SM is asked of the runtime (74, 33 and 15: groups of SMs are not multiples of eight).
 // In a graph, with 2 / 4 / 8 CTAs: rank 16, 1 token 8.7 / 6.0 / 4.9 us, 32 tiles 11.0 / 8.7 / 8.9, 64 (segments of 32 tokens) 13.2 / 13.0 / 18.2, 128 20.5 / 26.4 /
-// -; rank 64, 8 tiles 18.3 / 11.7 / 9.4, 18 11.5 / 8.5 / 14.6, 32 19.2 / 13.0 / 29.6, 128 28.7 / 32.9 / 86.
+// -; rank 64, 8 tiles 18.3 / 11.7 / 9.1, 18 11.5 / 8.5 / 14.6, 32 19.2 / 12.2 / 29.6, 128 28.5 / 32.9 / 86.
 template <typename T, int RT>
 int launch_adapters(llattn::AdapterParams& p, int npools, cudaStream_t stream) {
     using namespace llattn;
