@@ -154,7 +154,7 @@ def test_norm_does_not_depend_on_the_batch(api):
 
 @pytest.mark.gpu
 def test_norm_takes_columns_of_one_matrix(api, orc):
-    """x and delta side by side in one matrix, and a delta that is x itself."""
+    """x and delta side by side in one matrix."""
     x, d, gain = _inputs(40, 256, torch.float32, 3)
     both = torch.cat([torch.from_numpy(x), d], 1).cuda()
     q, s, qsum = torch.zeros((40, 256), dtype=torch.int8, device="cuda"), torch.zeros((40, 2), device="cuda"), torch.zeros((40, 2), dtype=torch.int32, device="cuda")
