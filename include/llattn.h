@@ -136,7 +136,7 @@ int llattn_dense_error_word(int** word);
  * q [T][K], s and sum [T][K/128] are the triple llattn_dense_w4a8 reads (q in fragment order), y [T][K] is fp16 or bf16 (y_type); either may be
  * NULL, not both. x is fp32, rows ldx values apart; delta (NULL: nothing is added, x is only read) is fp32, fp16 or bf16 (delta_type), rows ldd
  * values apart. K is a multiple of 128 up to 32,768; ldx and ldd are multiples of 4; x, delta, gain, q and y are 16-byte aligned. No output may
- * overlap another argument. The codes and sums are the same bits whatever T and the launch. A group that holds an infinity or NaN has codes
+ * overlap another argument (columns of one matrix may stand side by side as x and delta). The codes and sums are the same bits whatever T and the launch. A group that holds an infinity or NaN has codes
  * 0 and the scale NaN, and NaN anywhere in a row makes all of its scales NaN, so that a projection of it is NaN. A sum of squares beyond fp32
  * (values around 1e19) gives r = 0. The model's own norm rotates too (engine/ops.cu:116-135); no counterpart of this plain form there. */
 int llattn_add_norm_q8(float* x, int64_t ldx, const void* delta, int delta_type, int64_t ldd, const float* gain, float eps, int8_t* q,

@@ -173,6 +173,18 @@ inline bool overlap(const void* a, unsigned long long na, const void* b, unsigne
     const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return a && b && na && nb && x < y + nb && y < x + na;
 }
+// The same for two matrices of T rows each, of na and nb bytes, da and db bytes apart: columns of one matrix share no byte though their ranges overlap.
+inline bool rows_overlap(const void* a, long long na, long long da, const void* b, long long nb, long long db, long long T) {
+    const long long off = (long long)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));      // of b's first row from a's
+    if (!a || !b || off >= (T - 1) * da + na || -off >= (T - 1) * db + nb) return false;
+    // With equal distances the first and the last row of a have all the neighbours that any row has; else each row is looked at.
+    for (long long i = 0; i < T; i += da == db ? std::max(T - 1, 1ll) : 1) {
+        const long long behind = i * da - off - nb;                // the first row of b that ends behind the beginning of a's row
+        const long long j = behind < 0 ? 0 : behind / db + 1;
+        if (j < T && off + j * db < i * da + na) return true;
+    }
+    return false;
+}
 }  // namespace
 
 extern "C" int llattn_add_norm_q8(float* x, int64_t ldx, const void* delta, int delta_type, int64_t ldd, const float* gain, float eps, int8_t* q,
@@ -192,14 +204,16 @@ extern "C" int llattn_add_norm_q8(float* x, int64_t ldx, const void* delta, int 
         return fail(LLATTN_EINVAL, "add_norm_q8: x, delta, gain, q and y must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(s) % 4 || reinterpret_cast<uintptr_t>(sum) % 4) return fail(LLATTN_EINVAL, "add_norm_q8: s and sum must be 4-byte aligned");
     if (T == 0) return LLATTN_OK;
-    // (x and delta may be columns of one matrix: where rows are further apart than K, their ranges say nothing)
+    const long long esize = delta_type == LLATTN_F32 ? 4 : 2;
+    // (x and delta may be columns of one matrix, so it is their rows that count)
     struct { const void* p; unsigned long long n; bool out; } const m[] = {
-        {x, (unsigned long long)((T - 1) * ldx + K) * 4, delta != nullptr}, {delta, delta ? (unsigned long long)((T - 1) * ldd + K) * (delta_type == LLATTN_F32 ? 4 : 2) : 0, false},
+        {x, (unsigned long long)((T - 1) * ldx + K) * 4, delta != nullptr}, {delta, delta ? (unsigned long long)((T - 1) * ldd + K) * esize : 0, false},
         {gain, (unsigned long long)K * 4, false}, {q, (unsigned long long)T * K, true}, {s, (unsigned long long)T * K / 32, true},
         {sum, (unsigned long long)T * K / 32, true}, {y, (unsigned long long)T * K * 2, true}};
     for (int i = 0; i < 7; ++i)
         for (int j = 0; j < i; ++j)
-            if ((m[i].out || m[j].out) && !(j == 0 && i == 1 && (ldx > K || ldd > K)) && overlap(m[i].p, m[i].n, m[j].p, m[j].n)) return fail(LLATTN_EINVAL, "add_norm_q8: an output overlaps another argument");
+            if ((m[i].out || m[j].out) && overlap(m[i].p, m[i].n, m[j].p, m[j].n) && (i != 1 || rows_overlap(x, 4ll * K, 4 * ldx, delta, esize * K, esize * ldd, T)))
+                return fail(LLATTN_EINVAL, "add_norm_q8: an output overlaps another argument");
     int dev = 0, sms = 0;
     CU(cudaGetDevice(&dev));
     CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
