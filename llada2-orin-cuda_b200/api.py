@@ -385,7 +385,7 @@ def qkv_prepare_commit_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v,
         raise ValueError("a prefill pass commits whole 32-token blocks")
     if pages is None and cache.numel() < NKV * max_blocks * KV_BLOCK_BYTES:
         raise ValueError("the cache holds fewer than max_blocks blocks")
-    if cache.get_device() != dev or cache.element_size() != 1 or (pages is not None and (pages.get_device() != dev or pages.numel() != nb * NKV or pages.element_size() != 4)):
+    if cache.get_device() != dev or cache.element_size() != 1 or (pages is not None and (pages.get_device() != dev or pages.numel() != nb * NKV or pages.dtype is not _torch()[3])):
         _refuse("axes", "cache uint8, pages int32 [nb][4]", cache=cache, pages=pages)
     if T:
         _check(lib().llattn_qkv_prepare_commit_axes(*args, nb, _ptr(cache), _ptr(pages), max_blocks, blk, st))

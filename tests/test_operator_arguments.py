@@ -1,0 +1,47 @@
+"""What the binding of the newer operators hands to the C entry points, with CPU tensors and a recording library in the place of the real one: no
+launch, so calls whose arguments are wrong can be made."""
+import gc
+import importlib
+import weakref
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Recorder:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append((name, args)) or 0
+
+
+@pytest.fixture
+def api(pkg, monkeypatch):
+    m = importlib.import_module(pkg.__name__ + ".api")
+    types = {torch.float32: m.F32, torch.float16: m.F16, torch.bfloat16: m.BF16}
+    rec = Recorder()
+    monkeypatch.setattr(m, "_torch_of", (torch.float32, torch.float16, torch.int8, torch.int32, types, lambda: -1, lambda dev: 0))      # -1: the CPU's index
+    monkeypatch.setattr(m, "_lib", rec)
+    m.recorder = rec
+    return m
+
+
+def _producer(axes=3, T=32):
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype)
+    return dict(qkv=z(T, 6 * 512), pos=z(axes, T, dtype=torch.int32), axis_of=bytes([0] * 8 + [1] * 12 + [2] * 12), gq=z(128), gk=z(128), eps=1e-6, inv_freq_t=z(32),
+                q=z(T, 16, 128, dtype=torch.half), k=z(T, 4, 128, dtype=torch.half), v=z(T, 4, 128, dtype=torch.half))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.uint32, torch.int64, torch.int16])
+def test_pages_of_another_type_are_refused(api, dtype):
+    """Page indices are read as int32: the bits of floats would be indices far outside the pool."""
+    args, cache = _producer(), torch.zeros((4, 4736), dtype=torch.uint8)
+    pages = torch.arange(4).reshape(1, 4)
+    api.qkv_prepare_commit_axes(**args, cache=cache, pages=pages.to(torch.int32))
+    assert [name for name, _ in api.recorder.calls] == ["llattn_qkv_prepare_commit_axes"]
+    with pytest.raises(ValueError):
+        api.qkv_prepare_commit_axes(**args, cache=cache, pages=pages.to(dtype))
+    assert len(api.recorder.calls) == 1
