@@ -355,6 +355,8 @@ def _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream):
     f32, f16, _, i32, _, device, handle = _torch()
     dev, T = device(), qkv.shape[0]
     n = T * NKV * D
+    if type(axis_of) is not bytes:
+        axis_of = bytes(list(axis_of))       # (of an array itself: its memory, whatever the width of its numbers)
     if (qkv.dtype is not f32 or qkv.numel() != 6 * n or qkv.get_device() != dev or not qkv.is_contiguous() or
             pos.dtype is not i32 or pos.dim() != 2 or pos.shape[1] != T or pos.get_device() != dev or not pos.is_contiguous() or
             gq.dtype is not f32 or gq.numel() != D or gq.get_device() != dev or not gq.is_contiguous() or
@@ -366,7 +368,7 @@ def _axes_args(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream):
         _refuse("axes", "qkv fp32 [T][3072], pos int32 [axes][T], 32 axes, gq and gk fp32 [128], inv_freq fp32 [32], q fp16 [T][16][128], k and v fp16 [T][4][128]",
                 qkv=qkv, pos=pos, gq=gq, gk=gk, inv_freq=inv_freq_t, q=q, k=k, v=v)
     return T, dev, (handle(dev) if stream is None else _stream(stream)), (
-        qkv.data_ptr(), pos.data_ptr(), pos.shape[0], bytes(axis_of), gq.data_ptr(), gk.data_ptr(), eps, inv_freq_t.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr())
+        qkv.data_ptr(), pos.data_ptr(), pos.shape[0], axis_of, gq.data_ptr(), gk.data_ptr(), eps, inv_freq_t.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr())
 
 
 def qk_norm_rope_axes(qkv, pos, axis_of, gq, gk, eps, inv_freq_t, q, k, v, stream=None) -> None:

@@ -45,3 +45,20 @@ def test_pages_of_another_type_are_refused(api, dtype):
     with pytest.raises(ValueError):
         api.qkv_prepare_commit_axes(**args, cache=cache, pages=pages.to(dtype))
     assert len(api.recorder.calls) == 1
+
+
+@pytest.mark.parametrize("as_given", [bytes, bytearray, list, tuple, np.array, lambda a: np.array(a, np.int32), lambda a: np.array(a, np.uint8), torch.tensor])
+def test_axes_may_come_as_any_sequence(api, as_given):
+    """The axis of a frequency is what the sequence has there, not what the memory behind it has: arrays of wider numbers too."""
+    axes = [0, 2, 1, 1] * 8
+    args = dict(_producer(), axis_of=as_given(axes))
+    api.qk_norm_rope_axes(**args)
+    api.qkv_prepare_commit_axes(**args, cache=torch.zeros((4, 4736), dtype=torch.uint8), max_blocks=1)
+    assert [a[3] for _, a in api.recorder.calls] == [bytes(axes)] * 2
+
+
+@pytest.mark.parametrize("bad", [np.arange(32) - 1, [256] * 32, np.full(32, 0.5), list(range(31))])
+def test_axes_that_are_no_axes_are_refused(api, bad):
+    with pytest.raises((ValueError, TypeError)):
+        api.qk_norm_rope_axes(**dict(_producer(), axis_of=bad))
+    assert api.recorder.calls == []
