@@ -450,7 +450,8 @@ class AdapterPool:
 
 
 class AdapterPools:
-    """One to four pools for calls of adapters_w4a8, checked once; holds their tensors."""
+    """One to four pools for calls of adapters_w4a8, checked once; holds the memory of their tensors as they were then. Another tensor given to
+    a pool later is not seen: make new pools for it."""
 
     def __init__(self, pools: Sequence[AdapterPool]):
         self.pools = list(pools)
@@ -461,6 +462,7 @@ class AdapterPools:
         if any(t is not None and t.get_device() != self.device for p in self.pools for t in (p.A, p.B, p.scale, p.ranks)):
             raise ValueError("the pools are on one device")
         self._c = (_AdapterPool * len(self.pools))(*[p._c() for p in self.pools])
+        self._held = [t.detach() for p in self.pools for t in (p.A, p.B, p.scale, p.ranks) if t is not None]      # whose addresses _c has
         self._rows = max(p.row0 + p.B.shape[1] for p in self.pools)
 
 

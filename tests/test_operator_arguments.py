@@ -2,7 +2,6 @@
 launch, so calls whose arguments are wrong can be made."""
 import gc
 import importlib
-import weakref
 
 import numpy as np
 import pytest
@@ -62,3 +61,48 @@ def test_axes_that_are_no_axes_are_refused(api, bad):
     with pytest.raises((ValueError, TypeError)):
         api.qk_norm_rope_axes(**dict(_producer(), axis_of=bad))
     assert api.recorder.calls == []
+
+
+@pytest.mark.parametrize("name", ["A", "B", "scale", "ranks"])
+@pytest.mark.parametrize("how", ["attribute", "data", "pool"])
+def test_pools_keep_the_memory_they_call_with(api, name, how):
+    """The addresses of a call are those of the tensors at the check. A pool's field, a tensor's memory or the list of pools may change behind it: what
+    the addresses stand for lives as long as the pools, and takes the pools' next calls."""
+    def tensors():
+        return dict(A=torch.ones((3, 8, 128), dtype=torch.half), B=torch.ones((3, 4, 8), dtype=torch.half), scale=torch.ones(3), ranks=torch.ones(3, dtype=torch.int32))
+    first = tensors()
+    at = first[name].data_ptr()
+    pools = api.adapter_pools([api.AdapterPool(**first)])
+    pool = pools.pools[0]
+    if how == "attribute":
+        setattr(pool, name, tensors()[name])
+    elif how == "data":
+        first[name].data = tensors()[name]
+    else:
+        pools.pools.clear()
+    del first, pool
+    gc.collect()
+    assert getattr(pools._c[0], name) == at
+    assert any(t.data_ptr() == at for t in _held(pools)), "the memory behind a call's address is not held"
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype)
+    api.adapters_w4a8(pools, z(4, 128, dtype=torch.int8), z(4, 1), z(4, 4), z(2, dtype=torch.int32), z(1, dtype=torch.int32))
+    assert [n for n, _ in api.recorder.calls] == ["llattn_adapters_w4a8"]
+
+
+def _held(pools):
+    """The tensors that can be reached from the pools."""
+    seen, todo, found = set(), [vars(pools)], []
+    while todo:
+        x = todo.pop()
+        if id(x) in seen:
+            continue
+        seen.add(id(x))
+        if torch.is_tensor(x):
+            found.append(x)
+        elif isinstance(x, dict):
+            todo += x.values()
+        elif isinstance(x, (list, tuple)):
+            todo += x
+        elif hasattr(x, "A"):
+            todo.append(vars(x))
+    return found
