@@ -156,7 +156,8 @@ typedef struct llattn_adapter_pool {
 #define LLATTN_MAX_ADAPTER_POOLS 4
 
 /* The tokens [seg_first[i], seg_first[i + 1]) belong to segment i, whose adapter is seg_adapter[i] in every pool (both device arrays, nseg + 1
- * and nseg long, bounds ascending; -1, or an index that the pool does not have: none). For a token n of a segment with adapter a, and every pool:
+ * and nseg long, bounds ascending: one below an earlier one counts as that one, one outside 0 .. ntokens as the nearer of them; -1, or an index that the
+ * pool does not have: none). For a token n of a segment with adapter a, and every pool:
  *   Y[n][row0 + i] += scale[a] * sum_j B[a][i][j] * sum_k A[a][j][k] * s[n][k / 128] * q[n][k]
  * from the activations (q, s) that the projection itself reads. All sums are fp32, and 22 bits of the inner one go into the outer one; the result is
  * added to Y in the memory, rounded once (numbers below 2^-126 count as zero there; an infinite inner sum makes NaN). The order of the sums, and so

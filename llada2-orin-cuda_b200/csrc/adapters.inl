@@ -167,8 +167,8 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Where tile `want` is, the tiles of the segments being counted through in order: the segment's adapter, or -1, first token and tokens (0: there is no
-// such tile). Bounds that are out of range or not in order give no tokens. Every warp for itself, a lane for a run of neighbouring segments:
-// one load behind the launch, and no barrier.
+// such tile). A bound is cut to the tokens there are, and one below an earlier one counts as that one: a token is in one segment at most, and there
+// are no more tiles than the grid has. Every warp for itself, a lane for a run of neighbouring segments: one load behind the launch, and no barrier.
 struct AdapterPlace { int adapter, n0, live; };
 __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, int want, int lane) {
     const int per = (p.nseg + 31) / 32, s0 = min(lane * per, p.nseg), s1 = min(s0 + per, p.nseg);
@@ -176,10 +176,29 @@ __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, in
     auto tiles = [](int t0, int t1) { return t1 > t0 ? (t1 - t0 + AD_TOK - 1) / AD_TOK : 0; };
     int mine = 0, t0 = bound(s0);
     int a = s0 < s1 ? __ldg(p.adapter + s0) : -1;             // with up to 32 segments all there is to it
+    bool back = false;                         // a lane sees its run's bounds and the next run's first one: all neighbours
     for (int i = s0, t = t0; i < s1; ++i) {
         const int t1 = bound(i + 1);
+        back |= t1 < t;
         mine += tiles(t, t1);
         t = t1;
+    }
+    if (__any_sync(0xffffffffu, back)) {       // again, from the largest bound of the runs ahead
+        int most = t0;
+        for (int i = s0 + 1; i < s1; ++i) most = max(most, bound(i));
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, most, o);
+            if (lane >= o) most = max(most, v);
+        }
+        const int ahead = __shfl_up_sync(0xffffffffu, most, 1);
+        if (lane > 0) t0 = max(t0, ahead);
+        mine = 0;
+        for (int i = s0, t = t0; i < s1; ++i) {
+            const int t1 = max(t, bound(i + 1));
+            mine += tiles(t, t1);
+            t = t1;
+        }
     }
     int upto = mine;
 #pragma unroll
@@ -191,7 +210,7 @@ __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, in
     const bool found = k >= 0 && k < mine;
     if (found)
         for (int i = s0; i < s1; ++i) {
-            const int t1 = bound(i + 1), n = tiles(t0, t1);
+            const int t1 = max(t0, bound(i + 1)), n = tiles(t0, t1);
             if (k < n) {
                 if (i > s0) a = __ldg(p.adapter + i);
                 live = min(AD_TOK, t1 - t0 - AD_TOK * k);
