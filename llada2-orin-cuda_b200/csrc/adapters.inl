@@ -442,14 +442,26 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         }
     }
     if constexpr (C::WIDE) ptx::fence_proxy_async_smem();
-    ok = __syncthreads_and(ok);                // H is there; where sums are missing this CTA leaves Y as it is
+    ok = __syncthreads_and(ok);                // H is there
+    // Where sums are missing this CTA leaves Y as it is, says so, and stays until the others' stores into its shared memory are in: whatever its rank and rows.
+    if (!ok) {
+        cp_async_wait<0>();
+        if (tid == 0) {
+            atomicOr(&g_dense_err, ERR_WAIT_FOLD);
+            *abort_flag = 0;
+            ptx::mbar_wait(bar, 0, abort_flag);
+        }
+        __syncthreads();
+        if constexpr (C::WIDE)
+            if (warp == 0) ptx::tmem_dealloc(*reinterpret_cast<volatile uint32_t*>(ad_smem + 28), 256);
+        return;
+    }
     if constexpr (C::WIDE) {
         // ---- Y, 128 rows at a time on tcgen05: a tile of B times all parts of H beside one another into tensor memory
         ptx::tc_fence_after();
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 28);
         const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = ptx::idesc_f16(128, T::PARTS * AD_TOK, false, false) | T::IDESC;
         constexpr int COLS = AD_TOK / 2;       // of a warp: a quarter of the rows, half of the tokens
-        const bool wanted = rank != 0;
         const int nw = COLS * (warp >> 2);
         float2 down[COLS / 8];
 #pragma unroll
@@ -465,8 +477,8 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         fetch_b(first + C::WTILES - 1);        // the sums have been passed on
         cp_async_wait<C::WTILES - 1>();
         ptx::fence_proxy_async_smem();
-        ok = __syncthreads_and(ok && wanted && first < end);
-        if (ok) {
+        __syncthreads();
+        if (rank != 0 && first < end) {
             if (warp == 0) multiply(first);
             issued = 1;
         }
@@ -522,10 +534,8 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         }
         cp_async_wait<0>();
         ok = __syncthreads_and(ok);
-        if (tid == 0 && !ok && wanted && first < end) {
+        if (tid == 0 && !ok) {                 // products that are still on their way
             atomicOr(&g_dense_err, ERR_WAIT_FOLD);
-            *abort_flag = 0;
-            if (parts > 1) ptx::mbar_wait(bar, 0, abort_flag);                 // stores and products that are still on their way
             for (int k = max(0, issued - 2); k < issued; ++k) {
                 *abort_flag = 0;
                 ptx::mbar_wait(bar + 8 + 8 * (k & 1), (k >> 1) & 1, abort_flag);
@@ -534,15 +544,6 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         __syncthreads();
         if (warp == 0) ptx::tmem_dealloc(tmem, 256);
     } else {
-        if (!ok) {
-            if (tid == 0) {
-                atomicOr(&g_dense_err, ERR_WAIT_FOLD);
-                *abort_flag = 0;
-                ptx::mbar_wait(bar, 0, abort_flag);                            // stores that are still on their way here
-            }
-            __syncthreads();
-            return;
-        }
         if (rank == 0) return;
         // ---- Y, a warp for 32 rows and 32 tokens
 #pragma unroll 1
