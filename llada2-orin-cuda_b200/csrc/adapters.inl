@@ -14,11 +14,14 @@
 // in an m16n8k16 are given to just these, and A is read to match, eight bytes a lane. Groups of A, codes and scales come through cp.async, two to four
 // ahead.
 //
-// Second product: B is multiplied as it is, too, with H in parts: two of fp16 (22 bits, behind a power of two that brings the token's largest to 2^13)
-// or three of bf16 (24 bits). One part alone would leave 2^-11 or 2^-8 of the adapter's contribution, two of bf16 2^-17 = 8e-6, an order above the
-// rest of the sums' error. Up to 32 ranks with mma.sync, a warp for 32 rows: four for each of its eight row lanes, so that a token's 32 values
-// of Y are one 128-byte line and a lane adds 16 bytes of it. More ranks on tcgen05: 128 rows of B as the A operand, 64 or 96 columns of all parts of the
-// tokens' H as the B operand, B copied into the swizzled tile in an order of rows that gives a thread four neighbouring ones from tensor memory.
+// Second product: B is multiplied as it is, too, with H in parts that have all of its exponents: three of bf16 for bf16 (24 bits), two of tf32 for fp16 (22
+// bits), whose B is widened (11 bits, exact). One part alone would leave 2^-8 or 2^-11 of the adapter's contribution, two of bf16 2^-17 = 8e-6, an order
+// above the rest of the sums' error. Two of fp16 behind a power of two for the token, with fp16's B as it is, took 3 to 8 % less for 64 ranks (8 segments of
+// 128 tokens 12.2 us, now 13.2) and 10 % less for 128, but fp16 has five bits of exponent: a rank whose sum is 2^-24 of the token's largest kept 14 bits, one
+// of 2^-40 nothing, however much B makes of it. Up to 32 ranks with mma.sync, a warp for 32 rows: four for each of its eight row lanes, so that a token's
+// 32 values of Y are one 128-byte line and a lane adds 16 bytes of it. More ranks on tcgen05: 128 rows of B as the A operand, 64 or 96 columns of all
+// parts of the tokens' H as the B operand, B copied (or widened) into the swizzled tile in an order of rows that gives a thread four neighbouring ones
+// from tensor memory.
 // Y is added to by vector reductions in L2 and never comes to an SM: loading and storing it instead took 22 us in the place of 13 for 64 segments of 32 tokens.
 //
 // What bounds it: one token 4.9 us, a chain of launch, segment, operands, the cluster's exchange (1.2 us) and B. A full batch (64 segments of 32 tokens,
@@ -62,13 +65,8 @@ struct AdapterF16 {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
-    static constexpr uint32_t IDESC = 0;       // operand types of kind::f16
-    static constexpr int PARTS = 2;            // of H, in fp16: 22 bits of a value, the largest of a token brought to 2^13
-    static __device__ __forceinline__ uint32_t part(float& a, float& b) {      // two values rounded, what is left of them in their place
-        const half2 x = __floats2half2_rn(a, b);
-        a -= __low2float(x); b -= __high2float(x);
-        return *reinterpret_cast<const uint32_t*>(&x);
-    }
+    static constexpr bool TF32 = true;         // the second product's type,
+    static constexpr int PARTS = 2;            // and H's parts in it
 };
 struct AdapterBF16 {
     // a byte v behind 0x43 is the bf16 number 128 + (v & 127), and with its sign bit alone 128 or 256: their difference is v, exact
@@ -84,52 +82,72 @@ struct AdapterBF16 {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
-    static constexpr uint32_t IDESC = 1u << 7 | 1u << 10;
-    static constexpr int PARTS = 3;            // of H, in bf16: 24 bits, and no range to be kept
-    static __device__ __forceinline__ uint32_t part(float& a, float& b) {
+    static constexpr bool TF32 = false;
+    static constexpr int PARTS = 3;
+    static __device__ __forceinline__ uint32_t part(float& a, float& b) {      // two values rounded, what is left of them in their place
         const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
         a -= __low2float(x); b -= __high2float(x);
         return *reinterpret_cast<const uint32_t*>(&x);
     }
 };
-// 64 ranks: four K-steps of kind::f16 over 128-byte-swizzle tiles (A: 128 rows of B, B: the parts of the tokens' H). One elected lane issues.
-__device__ __forceinline__ void mma_f16_block_warp(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate_first) {
-    asm volatile(
-        "{\n\t.reg .pred pe, pf, pt;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
-        "elect.sync _|pe, 0xffffffff;\n\t"
-        "setp.ne.b32 pf, %5, 0;\n\t setp.eq.b32 pt, 0, 0;\n\t"
-        "mov.b64 da, {%1, %3};\n\t mov.b64 db, {%2, %3};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, pf;\n\t"
-        "add.u32 x, %1, 2;\n\t add.u32 y, %2, 2;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, pt;\n\t"
-        "add.u32 x, %1, 4;\n\t add.u32 y, %2, 4;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, pt;\n\t"
-        "add.u32 x, %1, 6;\n\t add.u32 y, %2, 6;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"
-        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, pt;\n\t"
-        "}\n" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate_first) : "memory");
+__device__ __forceinline__ float2 half2_floats(uint32_t w) { return __half22float2(*reinterpret_cast<const half2*>(&w)); }
+__device__ __forceinline__ float to_tf32(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return __uint_as_float(r);
 }
+__device__ __forceinline__ void mma_tf32(float (&c)[4], float a0, float a1, float a2, float a3, float b0, float b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)),
+          "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+// A block of 64 ranks in bf16 or 32 in tf32: four K-steps over 128-byte-swizzle tiles (A: 128 rows of B, B: the parts of the tokens' H). One elected lane issues.
+#define AD_MMA_BLOCK(KIND)                                                                                                                                    \
+    asm volatile(                                                                                                                                             \
+        "{\n\t.reg .pred pe, pf, pt;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"                                                                               \
+        "elect.sync _|pe, 0xffffffff;\n\t"                                                                                                                    \
+        "setp.ne.b32 pf, %5, 0;\n\t setp.eq.b32 pt, 0, 0;\n\t"                                                                                                \
+        "mov.b64 da, {%1, %3};\n\t mov.b64 db, {%2, %3};\n\t"                                                                                                 \
+        "@pe tcgen05.mma.cta_group::1.kind::" KIND " [%0], da, db, %4, pf;\n\t"                                                                               \
+        "add.u32 x, %1, 2;\n\t add.u32 y, %2, 2;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"                                                       \
+        "@pe tcgen05.mma.cta_group::1.kind::" KIND " [%0], da, db, %4, pt;\n\t"                                                                               \
+        "add.u32 x, %1, 4;\n\t add.u32 y, %2, 4;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"                                                       \
+        "@pe tcgen05.mma.cta_group::1.kind::" KIND " [%0], da, db, %4, pt;\n\t"                                                                               \
+        "add.u32 x, %1, 6;\n\t add.u32 y, %2, 6;\n\t mov.b64 da, {x, %3};\n\t mov.b64 db, {y, %3};\n\t"                                                       \
+        "@pe tcgen05.mma.cta_group::1.kind::" KIND " [%0], da, db, %4, pt;\n\t"                                                                               \
+        "}\n" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate_first) : "memory")
+template <bool TF32>
+__device__ __forceinline__ void mma_adapter_block_warp(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate_first) {
+    if constexpr (TF32) AD_MMA_BLOCK("tf32");
+    else AD_MMA_BLOCK("f16");
+}
+#undef AD_MMA_BLOCK
 // Sixteen bytes of which the first `bytes` are copied and the others become zeros.
 __device__ __forceinline__ void cp_async16_some(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // A CTA of RT sixteens of ranks and 32 tokens: its warps' shares and its shared memory.
-template <int RT> struct AdapterTile {
+template <int RT, bool TF32> struct AdapterTile {
     static constexpr int R = 16 * RT, TOK = AD_TOK;
     // First product: a warp takes RW x 4 tiles of (16 ranks, 8 tokens) and every WK-th run of sixteen values of a group
     static constexpr int RW = RT < 2 ? RT : 2, WR = RT / RW, WK = AD_WARPS / WR;
     // A stage: a group of A and of the codes, rows padded for conflict-free reads, and the tokens' scales
     static constexpr int LDA = 288, LDQ = 144, Q = R * LDA, SX = Q + TOK * LDQ, STAGE = SX + TOK * 4, STAGES = RT > 4 ? 2 : RT > 1 ? 3 : 5;
-    // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], and H in parts of 16 bits. For few ranks the first two parts [TOK]
-    // rows LDH bytes apart, and the third; else the tensor cores' tiles, 64 ranks a block, and behind them tiles of 128 rows of B, the last one where the sums were. A power of two for each
-    // token. In front of all a slot [TOK][R] for the sums of each other CTA of the cluster.
+    // Then, in the same place: the warps' sums by share of the group, [WK][TOK][LDP], and H in parts. For few ranks [TOK] rows LDH bytes apart (bf16: the
+    // first two parts side by side, then the third; tf32: one part, then the other); else the tensor cores' tiles, a block of ranks after the other, and behind them
+    // tiles of 128 rows of B, the last one where the sums were (of tf32 one tile: half of its blocks there, half behind H). In front of all a
+    // slot [TOK][R] for the sums of each other CTA of the cluster.
     static constexpr bool WIDE = RT >= 4;
-    static constexpr int LDP = R + 4, LDH = 4 * R + (RT == 2 ? 64 : 0), LDH3 = LDH / 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
-    static constexpr int BLOCKS = (R + 63) / 64, HBLOCK = 3 * TOK * 128, WBLOCK = 128 * 128, WTILE = BLOCKS * WBLOCK, WTILES = RT > 4 ? 2 : 3;
+    static constexpr int LDP = WIDE ? R : R + 4, LDH = 4 * R + (RT == 2 ? 64 : 0), LDH3 = LDH / 2, SLOT = R * TOK * 4, SUMS = WK * TOK * LDP * 4;
+    static constexpr int BLOCK = TF32 ? 32 : 64, BLOCKS = (R + BLOCK - 1) / BLOCK, HBLOCK = (TF32 ? 2 : 3) * TOK * 128, WBLOCK = 128 * 128, WTILE = BLOCKS * WBLOCK, WTILES = RT > 4 ? 2 : 3;
     static constexpr int H_AT = WIDE ? (SUMS + 1023) / 1024 * 1024 : SUMS, W_AT = H_AT + BLOCKS * HBLOCK;
-    static constexpr int UP_AT = WIDE ? W_AT + (WTILES - 1) * WTILE : H_AT + TOK * (LDH + LDH3), AREA = UP_AT + TOK * 4;
-    static_assert(!WIDE || WTILE <= H_AT, "the last tile takes the place of the sums");
+    static constexpr int AREA = !WIDE ? H_AT + TOK * (LDH + (TF32 ? LDH : LDH3)) : TF32 ? W_AT + WTILE / 2 : W_AT + (WTILES - 1) * WTILE;
+    static_assert(!WIDE || (TF32 ? WTILE / 2 : WTILE) <= H_AT, "the last tile takes the place of the sums");
     static __device__ __forceinline__ int tile_at(int i) { return i % WTILES == WTILES - 1 ? 0 : W_AT + i % WTILES * WTILE; }
+    static __device__ __forceinline__ int block_at(int k) { return k < BLOCKS / 2 ? k * WBLOCK : W_AT + (k - BLOCKS / 2) * WBLOCK; }      // of the one tile
+    // Where a token's sum of a rank is: the rows of a warp's stores are two apart (padded, or swizzled: its ranks in eights)
+    static __device__ __forceinline__ int sum_at(int row, int j) { return row * LDP + (WIDE ? j ^ ((row >> 1 & 3) << 3) : j); }
     static constexpr int HEAD = WIDE ? 1024 : 64;
     static constexpr int bytes(int ctas) { return HEAD + (ctas - 1) * SLOT + (STAGES * STAGE > AREA ? STAGES * STAGE : AREA); }
     static constexpr int MOST = bytes(8) <= 227 * 1024 ? 8 : 4;        // CTAs of a cluster
@@ -229,7 +247,7 @@ __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, in
 template <typename T, int RT>
 __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(1024) uint8_t ad_smem[];
-    using C = AdapterTile<RT>;
+    using C = AdapterTile<RT, T::TF32>;
     ptx::grid_dependency_wait();               // nothing is read or written before the kernel ahead has completed
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const AdapterPoolDesc& P = p.pool[blockIdx.y];
@@ -368,8 +386,41 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             }
         cp_async_commit();
     };
-    if constexpr (C::WIDE)
-        for (int c = first; c < first + C::WTILES - 1; ++c) fetch_b(c);
+    // The same of fp16, through registers: a thread's eight ranks of every 2048 / R-th row asked for, and put into the tile as fp32 numbers.
+    constexpr int ASKED = C::WIDE && T::TF32 ? C::R / 16 : 1;
+    uint4 raw[ASKED];
+    auto ask_b = [&](int c) {
+        const int j = tid % (C::R / 8) * 8;
+#pragma unroll
+        for (int m = 0; m < ASKED; ++m) {
+            const int row = 128 * c + m * (AD_THREADS * 8 / C::R) + tid / (C::R / 8);
+            raw[m] = c < end && row < P.rows && j < rank ? __ldg(reinterpret_cast<const uint4*>(B + size_t(row) * P.rank + j)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    auto put_b = [&]() {
+        // (every other block's lanes begin with their second four ranks: eight neighbouring lanes then store to all banks)
+        const int j = tid % (C::R / 8) * 8, left = rank - j, swap = j / 32 & 1;
+        uint32_t mask[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mask[k] = 2 * k + 1 < left ? 0xffffffffu : 2 * k < left ? 0xffffu : 0u;
+#pragma unroll
+        for (int m = 0; m < ASKED; ++m) {
+            const int r = m * (AD_THREADS * 8 / C::R) + tid / (C::R / 8), at = r / 32 * 32 + r / 4 % 8 + r % 4 * 8;
+            const uint32_t w[4] = {raw[m].x & mask[0], raw[m].y & mask[1], raw[m].z & mask[2], raw[m].w & mask[3]};
+            uint8_t* to = area + C::block_at(j / 32) + at * 128;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float2 a = half2_floats(swap ? w[2 - 2 * k] : w[2 * k]), b = half2_floats(swap ? w[3 - 2 * k] : w[2 * k + 1]);
+                *reinterpret_cast<float4*>(to + ((j % 32 / 4 + (k ^ swap) ^ (at & 7)) << 4)) = make_float4(a.x, a.y, b.x, b.y);
+            }
+        }
+        ptx::fence_proxy_async_smem();
+    };
+    if constexpr (C::WIDE) {
+        if constexpr (T::TF32) ask_b(first);
+        else
+            for (int c = first; c < first + C::WTILES - 1; ++c) fetch_b(c);
+    }
     float* sums = reinterpret_cast<float*>(area);
 #pragma unroll
     for (int r = 0; r < C::RW; ++r)
@@ -377,7 +428,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                sums[(wk * AD_TOK + 8 * nt + 2 * t + (e & 1)) * C::LDP + 16 * (C::RW * wr + r) + g + 8 * (e >> 1)] = h[r][nt][e];
+                sums[C::sum_at(wk * AD_TOK + 8 * nt + 2 * t + (e & 1), 16 * (C::RW * wr + r) + g + 8 * (e >> 1))] = h[r][nt][e];
     __syncthreads();
     // ---- four ranks of a token at a time: this CTA's sums, to a slot in every other CTA of the cluster, and all CTAs' in their order
     constexpr int QUADS = (C::R * AD_TOK / 4 + AD_THREADS - 1) / AD_THREADS;
@@ -391,7 +442,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         if (n < AD_TOK) {
 #pragma unroll
             for (int k = 0; k < C::WK; ++k) {
-                const float4 u = *reinterpret_cast<const float4*>(sums + (k * AD_TOK + n) * C::LDP + j);
+                const float4 u = *reinterpret_cast<const float4*>(sums + C::sum_at(k * AD_TOK + n, j));
                 own[m].x += u.x; own[m].y += u.y; own[m].z += u.z; own[m].w += u.w;
             }
             for (int k = 0; k < parts; ++k)
@@ -418,26 +469,27 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = j + e < rank ? v[e] * scale : 0.f;      // what A has behind the rank, whatever it is, does not count
-            if constexpr (T::PARTS == 2) {                         // the token's ranks are with R / 4 neighbouring lanes
-                float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+            if constexpr (T::TF32) {
+                float4 w[2];
+                w[0] = make_float4(to_tf32(x[0]), to_tf32(x[1]), to_tf32(x[2]), to_tf32(x[3]));
+                w[1] = make_float4(to_tf32(x[0] - w[0].x), to_tf32(x[1] - w[0].y), to_tf32(x[2] - w[0].z), to_tf32(x[3] - w[0].w));
 #pragma unroll
-                for (int o = 1; o < C::R / 4; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int e = most < INFINITY ? max(int(__float_as_uint(most) >> 23) - 127, -100) : 13;
-                const float up = __uint_as_float(uint32_t(127 + 13 - e) << 23);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] *= up;
-                if (j == 0) reinterpret_cast<float*>(area + C::UP_AT)[n] = __uint_as_float(uint32_t(127 - 13 + e) << 23);
-            }
-            uint32_t w[T::PARTS][2];
-#pragma unroll
-            for (int k = 0; k < T::PARTS; ++k) { w[k][0] = T::part(x[0], x[1]); w[k][1] = T::part(x[2], x[3]); }
-            if constexpr (C::WIDE) {
-#pragma unroll
-                for (int k = 0; k < T::PARTS; ++k)
-                    *reinterpret_cast<uint2*>(hs + j / 64 * C::HBLOCK + (AD_TOK * k + n) * 128 + ((j % 64 / 8 ^ (n & 7)) << 4) + j % 8 * 2) = make_uint2(w[k][0], w[k][1]);
+                for (int k = 0; k < 2; ++k) {
+                    if constexpr (C::WIDE) *reinterpret_cast<float4*>(hs + j / 32 * C::HBLOCK + (AD_TOK * k + n) * 128 + ((j % 32 / 4 ^ (n & 7)) << 4)) = w[k];
+                    else *reinterpret_cast<float4*>(hs + (AD_TOK * k + n) * C::LDH + 4 * j) = w[k];
+                }
             } else {
-                *reinterpret_cast<uint4*>(hs + n * C::LDH + 4 * j) = make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
-                if constexpr (T::PARTS == 3) *reinterpret_cast<uint2*>(hs + AD_TOK * C::LDH + n * C::LDH3 + 2 * j) = make_uint2(w[2][0], w[2][1]);
+                uint32_t w[3][2];
+#pragma unroll
+                for (int k = 0; k < 3; ++k) { w[k][0] = T::part(x[0], x[1]); w[k][1] = T::part(x[2], x[3]); }
+                if constexpr (C::WIDE) {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k)
+                        *reinterpret_cast<uint2*>(hs + j / 64 * C::HBLOCK + (AD_TOK * k + n) * 128 + ((j % 64 / 8 ^ (n & 7)) << 4) + j % 8 * 2) = make_uint2(w[k][0], w[k][1]);
+                } else {
+                    *reinterpret_cast<uint4*>(hs + n * C::LDH + 4 * j) = make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
+                    *reinterpret_cast<uint2*>(hs + AD_TOK * C::LDH + n * C::LDH3 + 2 * j) = make_uint2(w[2][0], w[2][1]);
+                }
             }
         }
     }
@@ -460,23 +512,28 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         // ---- Y, 128 rows at a time on tcgen05: a tile of B times all parts of H beside one another into tensor memory
         ptx::tc_fence_after();
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(ad_smem + 28);
-        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = ptx::idesc_f16(128, T::PARTS * AD_TOK, false, false) | T::IDESC;
+        const uint32_t dhi = ptx::desc_hi(1024) | (2u << 29), idesc = ptx::idesc_f16(128, T::PARTS * AD_TOK, false, false) | (T::TF32 ? 2u << 7 | 2u << 10 : 1u << 7 | 1u << 10);      // tf32 or bf16
         constexpr int COLS = AD_TOK / 2;       // of a warp: a quarter of the rows, half of the tokens
         const int nw = COLS * (warp >> 2);
-        float2 down[COLS / 8];
-#pragma unroll
-        for (int i = 0; i < COLS / 8; ++i) down[i] = T::PARTS == 2 ? *reinterpret_cast<const float2*>(area + C::UP_AT + 4 * (nw + 8 * i + 2 * t)) : make_float2(1.f, 1.f);
         int issued = 0;
         auto multiply = [&](int c) {           // by warp 0
-            const uint32_t tile = area_s + C::tile_at(c - first), acc = tmem + ((c - first) & 1) * 128;
+            const uint32_t acc = tmem + ((c - first) & 1) * 128;
 #pragma unroll
-            for (int k = 0; k < C::BLOCKS; ++k)
-                mma_f16_block_warp(acc, ptx::desc_lo(tile + k * C::WBLOCK, 16), ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16), dhi, idesc, k > 0);
+            for (int k = 0; k < C::BLOCKS; ++k) {
+                const uint32_t tile = area_s + (T::TF32 ? C::block_at(k) : C::tile_at(c - first) + k * C::WBLOCK);
+                mma_adapter_block_warp<T::TF32>(acc, ptx::desc_lo(tile, 16), ptx::desc_lo(ptx::smem_u32(hs) + k * C::HBLOCK, 16), dhi, idesc, k > 0);
+            }
             ptx::mma_commit_warp(bar + 8 + 8 * ((c - first) & 1));
         };
-        fetch_b(first + C::WTILES - 1);        // the sums have been passed on
-        cp_async_wait<C::WTILES - 1>();
-        ptx::fence_proxy_async_smem();
+        // (the sums have been passed on)
+        if constexpr (T::TF32) {
+            put_b();
+            ask_b(first + 1);
+        } else {
+            fetch_b(first + C::WTILES - 1);
+            cp_async_wait<C::WTILES - 1>();
+            ptx::fence_proxy_async_smem();
+        }
         __syncthreads();
         if (rank != 0 && first < end) {
             if (warp == 0) multiply(first);
@@ -485,7 +542,10 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
         // the products of the next rows run while these rows' are on their way to Y: two accumulators (8 segments of 128 tokens of rank 64 13.0 -> 12.2 us)
 #pragma unroll 1
         for (int c = first; c < end && issued; ++c) {
-            if (c + 1 < end) {
+            if constexpr (T::TF32) {
+                ok = ptx::mbar_wait_warp(bar + 8 + 8 * ((c - first) & 1), ((c - first) >> 1) & 1, abort_flag);
+                if (ok && c + 1 < end) put_b();              // the tile has been read
+            } else if (c + 1 < end) {
                 cp_async_wait<C::WTILES - 2>();
                 ptx::fence_proxy_async_smem();
             }
@@ -497,9 +557,12 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
                 if (warp == 0) multiply(c + 1);
                 ++issued;
             }
-            ok = ptx::mbar_wait_warp(bar + 8 + 8 * ((c - first) & 1), ((c - first) >> 1) & 1, abort_flag);
-            ptx::tc_fence_after();
-            fetch_b(c + C::WTILES);            // in the place of the tile just used
+            if constexpr (T::TF32) ask_b(c + 2);
+            else {
+                ok = ptx::mbar_wait_warp(bar + 8 + 8 * ((c - first) & 1), ((c - first) >> 1) & 1, abort_flag);
+                ptx::tc_fence_after();
+                fetch_b(c + C::WTILES);        // in the place of the tile just used
+            }
             // rows 4 g and + 1 in the first, + 2 and + 3 in the second; tokens 8 i + 2 t and + 1; a part 32 columns behind the other
             uint32_t ra[T::PARTS][COLS / 2], rb[T::PARTS][COLS / 2];
             const int row = 128 * c + 32 * (warp & 3) + 4 * g;
@@ -515,11 +578,11 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
                 ptx::tmem_wait_ld_tied(rb[k]);
             }
             ptx::tc_fence_before();
-            auto sum = [&](uint32_t (&r)[T::PARTS][COLS / 2], int i, float by) {
+            auto sum = [&](uint32_t (&r)[T::PARTS][COLS / 2], int i) {
                 float v = __uint_as_float(r[T::PARTS - 1][i]);
 #pragma unroll
                 for (int k = T::PARTS - 2; k >= 0; --k) v += __uint_as_float(r[k][i]);
-                return T::PARTS == 2 ? v * by : v;
+                return v;
             };
             float* yrow = p.Y + (n0 + nw) * p.ldy + P.row0 + row;
             if (ok && row < P.rows)
@@ -528,8 +591,7 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int n = 8 * i + 2 * t + e;
-                        const float by = e ? down[i].y : down[i].x;
-                        if (nw + n < live) add_to4(yrow + n * p.ldy, sum(ra, 4 * i + e, by), sum(ra, 4 * i + 2 + e, by), sum(rb, 4 * i + e, by), sum(rb, 4 * i + 2 + e, by));
+                        if (nw + n < live) add_to4(yrow + n * p.ldy, sum(ra, 4 * i + e), sum(ra, 4 * i + 2 + e), sum(rb, 4 * i + e), sum(rb, 4 * i + 2 + e));
                     }
         }
         cp_async_wait<0>();
@@ -563,30 +625,42 @@ __global__ void __launch_bounds__(AD_THREADS, RT == 1 ? 3 : 2) adapters_kernel(c
                 for (int i = 0; i < 4; ++i) { w[i][0] = braw[i].x & m0; w[i][1] = braw[i].y & m1; }
                 const bool last = 16 * rt + 16 >= rank;
                 if (!last || c + AD_WARPS < end) load_b(braw, last ? c + AD_WARPS : c, last ? 0 : rt + 1);
-                uint4 x[4];
-                uint2 z[4];
-#pragma unroll
-                for (int nt = 0; nt < 4; ++nt) {
-                    x[nt] = *reinterpret_cast<const uint4*>(hs + (8 * nt + g) * C::LDH + 4 * j);
-                    if constexpr (T::PARTS == 3) z[nt] = *reinterpret_cast<const uint2*>(hs + AD_TOK * C::LDH + (8 * nt + g) * C::LDH3 + 2 * j);
-                }
                 // the smallest part first; no product right behind another one into the same accumulator
+                if constexpr (T::TF32) {
+                    float2 f[4][2];
 #pragma unroll
-                for (int k = T::PARTS - 1; k >= 0; --k)
+                    for (int i = 0; i < 4; ++i) { f[i][0] = half2_floats(w[i][0]); f[i][1] = half2_floats(w[i][1]); }
 #pragma unroll
-                    for (int nt = 0; nt < 4; ++nt)
+                    for (int k = 1; k >= 0; --k) {
+                        float4 x[4];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            T::mma(acc[i][nt], w[2 * i][0], w[2 * i + 1][0], w[2 * i][1], w[2 * i + 1][1], k == 2 ? z[nt].x : k ? x[nt].z : x[nt].x,
-                                   k == 2 ? z[nt].y : k ? x[nt].w : x[nt].y);
-            }
-            if constexpr (T::PARTS == 2)
+                        for (int nt = 0; nt < 4; ++nt) x[nt] = *reinterpret_cast<const float4*>(hs + (AD_TOK * k + 8 * nt + g) * C::LDH + 4 * j);
 #pragma unroll
-                for (int nt = 0; nt < 4; ++nt) {
-                    const float2 u = *reinterpret_cast<const float2*>(area + C::UP_AT + 4 * (8 * nt + 2 * t));
+                        for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) { acc[i][nt][0] *= u.x; acc[i][nt][1] *= u.y; acc[i][nt][2] *= u.x; acc[i][nt][3] *= u.y; }
+                            for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+                                    mma_tf32(acc[i][nt], f[2 * i][half].x, f[2 * i + 1][half].x, f[2 * i][half].y, f[2 * i + 1][half].y, half ? x[nt].z : x[nt].x, half ? x[nt].w : x[nt].y);
+                    }
+                } else {
+                    uint4 x[4];
+                    uint2 z[4];
+#pragma unroll
+                    for (int nt = 0; nt < 4; ++nt) {
+                        x[nt] = *reinterpret_cast<const uint4*>(hs + (8 * nt + g) * C::LDH + 4 * j);
+                        z[nt] = *reinterpret_cast<const uint2*>(hs + AD_TOK * C::LDH + (8 * nt + g) * C::LDH3 + 2 * j);
+                    }
+#pragma unroll
+                    for (int k = 2; k >= 0; --k)
+#pragma unroll
+                        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                T::mma(acc[i][nt], w[2 * i][0], w[2 * i + 1][0], w[2 * i][1], w[2 * i + 1][1], k == 2 ? z[nt].x : k ? x[nt].z : x[nt].x,
+                                       k == 2 ? z[nt].y : k ? x[nt].w : x[nt].y);
                 }
+            }
             if (!mine) continue;
             float* yrow = p.Y + n0 * p.ldy + P.row0 + row;
 #pragma unroll
@@ -611,7 +685,7 @@ namespace {
 template <typename T, int RT>
 int launch_adapters(llattn::AdapterParams& p, int npools, cudaStream_t stream) {
     using namespace llattn;
-    using C = AdapterTile<RT>;
+    using C = AdapterTile<RT, T::TF32>;
     constexpr int ONE_AN_SM = 200 * 1024, TWO_AN_SM = 113 * 1024;
     static std::mutex mu;
     static int clusters[64][3];                // by device; the first one 0: not asked yet
