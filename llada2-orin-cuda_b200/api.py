@@ -290,8 +290,8 @@ def dense_preview(rows: int, K: int, ntokens: int, num_sms: int):
 
 
 def dense_status(stream=None) -> int:
-    """0, or LlattnError (EDEVICE) when a wait of a dense_w4a8 call without an err_word ran out on the current device since the
-    last dense_status. Synchronises `stream`; call it where a step's results are read."""
+    """0, or LlattnError (EDEVICE) when a wait of a dense_w4a8 call without an err_word, or of an adapters_w4a8 call, ran out on the current
+    device since the last dense_status. Synchronises `stream`; call it where a step's results are read."""
     code = c_int(0)
     _check(lib().llattn_dense_status(_stream(stream), byref(code)))
     return code.value

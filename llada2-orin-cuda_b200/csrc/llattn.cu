@@ -459,7 +459,7 @@ int llattn_dense_status(void* stream, int* code) {
     if (*code) {
         const int zero = 0;
         CU(cudaMemcpyToSymbol(llattn::g_dense_err, &zero, sizeof(int)));
-        return fail(LLATTN_EDEVICE, "a projection's wait ran out (error bits 0x%x): its Y is incomplete", *code);
+        return fail(LLATTN_EDEVICE, "a wait of a projection or of its adapters ran out (error bits 0x%x): its Y is incomplete", *code);
     }
     return LLATTN_OK;
 }

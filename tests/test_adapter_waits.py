@@ -7,6 +7,8 @@ import importlib
 import os
 import re
 
+import pytest
+
 EXCHANGE = "ok = ptx::mbar_wait(bar, 0, abort_flag);"
 MARKS = ["cp_async_wait<0>()", "atomicOr(&g_dense_err, ERR_WAIT_FOLD)", "*abort_flag = 0", "ptx::mbar_wait(bar, 0, abort_flag)", "__syncthreads()", "ptx::tmem_dealloc(", "return;"]
 
@@ -70,3 +72,17 @@ def test_the_check_itself():
     assert _misses(good.replace("f();", "if (rank == 0) return;"))
     assert _misses(good.replace("ptx::mbar_wait(bar, 0, abort_flag); __", "__"))
     assert _misses(good.replace("*abort_flag = 0", "if (first < rows) *abort_flag = 0"))
+
+
+@pytest.mark.gpu
+def test_the_report_names_the_adapters(pkg):
+    """They share the projection's word, so its text must not send the reader to the projection alone. (The codes come from the wait self-test.)"""
+    torch = pytest.importorskip("torch")
+    api = importlib.import_module(pkg.__name__ + ".api")
+    assert api.dense_status() == 0
+    waited = torch.zeros(6, dtype=torch.int64, device="cuda")
+    api._check(api.lib().llattn_wait_selftest(1_000_000, api.dense_error_word(), waited.data_ptr(), None))
+    torch.cuda.synchronize()
+    with pytest.raises(api.LlattnError, match="projection or of its adapters"):
+        api.dense_status()
+    assert api.dense_status() == 0
