@@ -26,9 +26,12 @@ def _call(api, orc, T, first, adapter, rank=RANK):
     x = q[:, at].double() * s.double().repeat_interleave(128, 1)
     want = Y.double()
     ends = np.maximum.accumulate(np.clip(np.asarray(first), 0, T))
+    whose = np.full(T, -1)
     for t0, t1, a in zip(ends[:-1], ends[1:], adapter):
-        if 0 <= a < N and t1 > t0:
-            want[t0:t1] += x[t0:t1] @ A[a].double().t() @ B[a].double().t()
+        whose[t0:t1] = a
+    for a in range(N):
+        mine = torch.from_numpy(np.flatnonzero(whose == a)).cuda()
+        want[mine] += x[mine] @ A[a].double().t() @ B[a].double().t()
     assert float(want.abs().max()) < 2 ** 21
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
     api.adapters_w4a8(api.adapter_pools([api.AdapterPool(A, B)]), q, s, Y, i32(first), i32(adapter))
@@ -56,4 +59,15 @@ def test_many_bounds_that_go_back(api, orc, T, nseg, rank, kind):
         else:
             first = np.concatenate([first[::3], first[1::3], first[2::3]])
     got, want = _call(api, orc, T, [int(v) for v in first], [int(v) for v in r.integers(-1, N, nseg)], rank)
+    assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("rank", [8, 64])
+def test_the_most_segments(api, orc, rank):
+    """65,536 segments of one token, a few of them empty and one bound far back."""
+    T = nseg = 1 << 16
+    first = list(range(nseg + 1))
+    first[7] = first[9] = 9
+    first[40000] = 3
+    got, want = _call(api, orc, T, first, [i % (N + 1) - 1 for i in range(nseg)], rank)
     assert torch.equal(got.double(), want)
