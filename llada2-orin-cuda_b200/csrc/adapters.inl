@@ -24,10 +24,11 @@
 // from tensor memory.
 // Y is added to by vector reductions in L2 and never comes to an SM: loading and storing it instead took 22 us in the place of 13 for 64 segments of 32 tokens.
 //
-// What bounds it: one token 4.9 us, a chain of launch, segment, operands, the cluster's exchange (1.2 us) and B. A full batch (64 segments of 32 tokens,
-// adapters of rank 16) 13.0 us = 3.5 TB/s cold and 10.0 warm, of which 9.1 without the additions to Y: reading, computing and adding
-// overlap only across CTAs, and the chip holds all of them at once. 4096 tokens of rank 64 28.5 us, issue slots and shared memory of the first product
-// (45 %), the second product's tiles (the rest); with tf32 pairs on mma.sync 45, with one CTA a tile and every operand from memory 205.
+// What bounds it is the length of a CTA's chain at two CTAs of eight warps an SM (three for 16 ranks). One token 4.9 us: launch, segment, operands, the
+// cluster's exchange (1,600 of 8,000 cycles) and B. A full batch (64 segments of 32 tokens, adapters of rank 16) 13.3 us cold and 10.0 warm, 9.1 without the
+// additions to Y: 256 CTAs work at once (as many more find no tile and leave), 19,000 cycles each, of which 3,400 to find the segment, 4,700 in the first
+// product and 6,000 in the second; DRAM is at a quarter of its rate. 4096 tokens of rank 64 27.5 us, 38,000 cycles: 12,500 in the first product, 17,000 in
+// the second; issue slots 42 %, shared memory 30 %, tensor cores 11 %. With tf32 pairs on mma.sync 45, with one CTA a tile and every operand from memory 205.
 #pragma once
 
 namespace llattn {
@@ -187,6 +188,8 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // Where tile `want` is, the tiles of the segments being counted through in order: the segment's adapter, or -1, first token and tokens (0: there is no
 // such tile). A bound is cut to the tokens there are, and one below an earlier one counts as that one: a token is in one segment at most, and there
 // are no more tiles than the grid has. Every warp for itself, a lane for a run of neighbouring segments: one load behind the launch, and no barrier.
+// Every CTA looks at all bounds, so the search grows with their square: segments of one token (rank 16, K and rows 2048) 128 12.8 us, 512 43, 1024 102, 4096
+// 775, 10,000 1.7 ms, 65,536 136 ms, where the bytes of the largest take 0.19.
 struct AdapterPlace { int adapter, n0, live; };
 __device__ __forceinline__ AdapterPlace adapter_place(const AdapterParams& p, int want, int lane) {
     const int per = (p.nseg + 31) / 32, s0 = min(lane * per, p.nseg), s1 = min(s0 + per, p.nseg);

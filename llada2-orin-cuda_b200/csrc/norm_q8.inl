@@ -11,7 +11,9 @@
 // A lane holds four neighbouring values of a group (a run of four stays together in fragment order), a warp the group: maximum and code sum
 // are one redux instruction each. W warps share a row, group by group in turn; the row's sum of squares is folded lane-wise over a warp's
 // groups, by a butterfly over the lanes and over the warps in order, all in fp32.
-// Bound by memory from a few thousand rows on (8191 x 2048 with an fp32 addend 37.9 us = 5.8 TB/s), below by the launch and one round trip.
+// Bound by memory from a few thousand rows on (8191 x 2048 with an fp32 addend 37.9 us = 5.8 TB/s), below by the launch and one round trip. The 16-bit copy comes from
+// registers where a warp has all of its groups there (rows to 2048 values with 16 or 8 warps a row, to 512 with 4 or 2); beyond that the row and the gain are
+// read again, mostly from L2: 8191 x 2048 with a bf16 copy too 46.2 us, its bytes 38.5; 515 x 5120 with an addend and a copy 10.2, its bytes 5.3.
 #pragma once
 
 namespace llattn {
@@ -158,7 +160,10 @@ namespace {
 // How a row is shared. Few rows, or long ones: many warps a row, so that the chip is filled and the chain of a warp short. Many rows: few warps a row, each
 // with several groups of loads in flight. In a graph, rows x K, with 16 / 8 / 4 / 2 warps a row: 1 x 2048 2.0 / 2.4 / 3.1 / 6.0 us, 256 x 2048 2.8 / 2.9 /
 // 3.6 / 6.9, 512 x 2048 4.7 / 3.9 / 5.4 / 7.9, 515 x 5120 11.2 / 10.1 / 13.4 / 22.9, 1024 x 2048 7.8 / 8.1 / 7.3 / 10.2, 2048 x 2048 13.2 / 13.1 / 12.5 / 13.3,
-// 8191 x 2048 46.7 / 41.3 / 39.9 / 37.9, 2000 x 512 9.0 / 7.1 / 4.4 / 3.9, 2048 x 8192 36.2 / 39.2 / 42.4 / 45.1.
+// 8191 x 2048 46.7 / 41.3 / 39.9 / 37.9, 2000 x 512 9.0 / 7.1 / 4.4 / 3.9, 2048 x 8192 36.2 / 39.2 / 42.4 / 45.1. Between 4096 and 8064 values (fp16 addend): 700 x 4096
+// 9.0 / 11.5 / 10.9 / 17.7, 1024 x 4096 12.2 / 13.0 / 12.6 / 18.9, 4096 x 4096 38.5 / 37.9 / 38.1 / 43.6 and without an addend 30.9 / 25.6 / 26.8 / 29.5, 2000 x 6144 28.4 /
+// 30.1 / 32.4 / 34.3, 4096 x 8064 69.2 / 69.4 / 72.8 / 89.4: 8 for all of them, best for thousands of rows, up to 3 us behind 16 for a few rows an SM (700 x 7168
+// of fp32 14.7 / 17.6).
 template <int DTYPE>
 cudaError_t launch_norm_q8(const llattn::NormQ8Params& p, int sms, cudaStream_t stream) {
     const int groups = p.K / llattn::NQ_GROUP;
