@@ -159,7 +159,7 @@ typedef struct llattn_adapter_pool {
  * and nseg long, bounds ascending: one below an earlier one counts as that one, one outside 0 .. ntokens as the nearer of them; -1, or an index that the
  * pool does not have: none). For a token n of a segment with adapter a, and every pool:
  *   Y[n][row0 + i] += scale[a] * sum_j B[a][i][j] * sum_k A[a][j][k] * s[n][k / 128] * q[n][k]
- * from the activations (q, s) that the projection itself reads. All sums are fp32, and 22 bits of each inner one, whatever the others are, go into
+ * from the activations (q, s) that the projection itself reads. All sums are fp32, and 22 bits of each inner one above 2^-100, whatever the others are, go into
  * the outer one; the result is added to Y in the memory, rounded once (numbers below 2^-126 count as zero there; an infinite inner sum or B makes NaN). The order of the sums, and so
  * the bits, depends on ntokens, nseg, npools, K, the pools' sizes and the device only. Y has ldy values a row (a multiple of 4, at least row0 + rows); tokens
  * outside the segments, and of a segment without an adapter, keep theirs. q and Y are 16-byte aligned. `pools` is a host array of 1 to 4 pools
